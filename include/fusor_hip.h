@@ -305,6 +305,57 @@ fh_status fh_flash_attention_decode_static(fh_device *dev, int32_t q_dtype, int3
                                            int64_t kv_sh, int64_t kv_st, int32_t hq, int32_t hkv, int32_t d,
                                            float scale, int32_t skv, void *out_dev);
 
+/* -------------------------------------------------------------------- paged KV cache
+ * A cache of many sequences in pages of `page_size` positions (a power of two, 16 .. 4096) that the caller hands out:
+ * element c of position t of KV head h in page p lies at p * page_stride + h * head_stride + t * slot_stride + c of
+ * k_pages / v_pages (elements, K and V alike; rows of multiples of 16 bytes that do not overlap, [page][head][slot] or
+ * [page][slot][head]).  The pages are the caller's memory: nothing is allocated or kept here.  No counterpart in the
+ * reference, whose cache is one dense sequence (fusor-ml/fusor/src/cache/kv_cache.rs:24-63).
+ *   rows     tokens of all sequences one after the other: starts_dev[i] .. starts_dev[i + 1] - 1 are the new ones of
+ *            sequence i (i32, seqs + 1 of them, not decreasing; NULL: one row each).  Rows before the first and behind the
+ *            last sequence are left as they were, in the pages and in the outputs.
+ *   lens_dev positions of every sequence, its new rows among them (i32): row r has position
+ *            lens[i] - (starts[i + 1] - r).
+ *   table_dev [seqs, table_cols] i32: the page of positions n * page_size .. is table[i][n].  An entry that is no page
+ *            (below 0, or `pages` and above) is a hole: what is appended there is dropped, and nothing sees its positions,
+ *            nor those behind the table's last column.  So a sequence that only looks back a window may give pages back.
+ * dtype is the type of q, k, v and out, kv_dtype that of the pages: FH_F32, FH_F16 or FH_DECODER_BF16, both alike or f32
+ * rows over 16-bit pages.  head_dim is a multiple of 8 up to 256.  All sums and softmax statistics are f32.
+ * Lengths, starts and tables are read on the device when the call runs: a captured graph takes what they hold at replay. */
+
+/* q and k turned by their positions (RopeCache::forward{,_interleaved}, fusor-ml/fusor/src/composite/rope.rs:284-329; with
+ * several axes as models/kalosm-llama/src/raw/rope.rs does for pictures), k and v written to their pages.  q is
+ * [tokens, hq, d] with strides q_st (row) and q_sh (head) in elements, k and v are [tokens, hkv, d] with kv_st and kv_sh;
+ * q_out is contiguous [tokens, hq, d].  q and q_out may be NULL (append only), and cos and sin (nothing turns).
+ * cos / sin: [table_rows, table_pairs] f32.  Pair j of a head takes column j of the row that its axis' position names:
+ * sections_host[axes] (1 .. 4 axes) says how many pairs follow each axis, the first ones axis 0; NULL with one axis: all
+ * table_pairs.  What the sections leave of a head is not turned.  positions_dev: [axes, tokens] i32, NULL with one axis: the
+ * position in the cache.  interleaved: pairs are (2j, 2j + 1), otherwise (j, j + n) of n turned pairs.  Products are f32, each
+ * rounded on its own, results rounded once to their type.
+ * A row whose position has no page, or any of whose axes' positions lies outside the tables, is dropped: neither the
+ * pages nor its row of q_out are written.  q_out may be q itself where that is contiguous. */
+fh_status fh_paged_rope_append(fh_device *dev, int32_t dtype, int32_t kv_dtype, const void *q_dev, int64_t q_st,
+                               int64_t q_sh, const void *k_dev, const void *v_dev, int64_t kv_st, int64_t kv_sh, int32_t hq,
+                               int32_t hkv, int32_t d, const float *cos_dev, const float *sin_dev, int32_t table_rows,
+                               int32_t table_pairs, const int32_t *positions_dev, const int32_t *sections_host, int32_t axes,
+                               int32_t interleaved, void *k_pages_dev, void *v_pages_dev, int64_t page_stride,
+                               int64_t head_stride, int64_t slot_stride, int32_t pages, int32_t page_size,
+                               const int32_t *starts_dev, const int32_t *lens_dev, const int32_t *table_dev,
+                               int32_t table_cols, int32_t seqs, int32_t tokens, void *q_out_dev);
+/* softmax(q . K^T * scale) . V over the pages, causal: the row of position p sees the positions j <= p of its sequence, with
+ * window > 0 only those with j > p - window.  q is [tokens, hq, d] with strides q_st and q_sh (elements), out contiguous
+ * [tokens, hq, d]; query head h reads KV head h / (hq / hkv).  A row that sees nothing gets zeros.
+ * max_new: the most rows a sequence has; of sequences with more, the first max_new are computed and the rest left as they
+ * were.  With 1 (a decode step) every cache is split over the device and joined in the same launch; with more the rows run on
+ * the tiles of a prompt.  max_len: the longest sequence, or 0 where the host does not know; it chooses between forms of the
+ * kernels and nothing else.  Results do not depend on which pages hold a sequence. */
+fh_status fh_paged_attention(fh_device *dev, int32_t dtype, int32_t kv_dtype, const void *q_dev, int64_t q_st, int64_t q_sh,
+                             int32_t hq, int32_t hkv, int32_t d, float scale, int32_t window, const void *k_pages_dev,
+                             const void *v_pages_dev, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                             int32_t pages, int32_t page_size, const int32_t *starts_dev, const int32_t *lens_dev,
+                             const int32_t *table_dev, int32_t table_cols, int32_t seqs, int32_t tokens, int32_t max_new,
+                             int32_t max_len, void *out_dev);
+
 /* -------------------------------------------------------------------- glue
  * silu(g) * u, fusor-ml/fusor/src/composite/activations.rs:47-65 + raw/attention_layer.rs:195 */
 fh_status fh_swiglu(fh_device *dev, const float *gate_dev, const float *up_dev, float *y_dev,

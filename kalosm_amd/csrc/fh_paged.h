@@ -1,0 +1,48 @@
+// A paged key-value cache as kernels see it: which rows belong to which sequence, and where its positions lie.
+#pragma once
+#include "fh_internal.h"
+
+typedef _Float16 fh_half;
+typedef __bf16 fh_bf;
+
+enum { FH_PAGED_BF16 = FH_DECODER_BF16, FH_PAGED_MAX = 1 << 30 /* positions of a sequence */ };
+
+struct PagedKv {
+    const char *k, *v;
+    int64_t page, head, slot; // strides in bytes, K and V alike
+    int pages, shift;         // page_size = 1 << shift, 16 .. 4096
+};
+struct PagedRows {
+    const int *starts, *lens, *table; // starts NULL: one row a sequence
+    int cols, seqs, tokens, max_new;
+};
+struct PagedSeq {
+    int row, rows; // rows of q and out: row .. row + rows - 1, all of them inside the tensors whatever `starts` holds
+    int first;     // position of the first of them (below 0 where the sequence is said to be shorter than its new rows)
+    int len;       // positions that can be read: no further than the table's row reaches
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedRows &r, int shift, int i) {
+    PagedSeq s;
+    int len = r.lens[i], from = i, to = i + 1;
+    if (r.starts) from = r.starts[i], to = r.starts[i + 1];
+    len = len < 0 ? 0 : len > FH_PAGED_MAX ? FH_PAGED_MAX : len;
+    from = from < 0 ? 0 : from > r.tokens ? r.tokens : from;
+    to = to < from ? from : to > r.tokens ? r.tokens : to;
+    s.row = from;
+    s.first = len - (to - from);
+    s.rows = to - from < r.max_new ? to - from : r.max_new;
+    const int64_t reach = (int64_t)r.cols << shift;
+    s.len = len < reach ? len : (int)reach;
+    return s;
+}
+
+// Arguments both entry points check, without touching a device: FH_OK, or an error with its message.  `kv` and `rows` are filled in.
+fh_status fh_paged_arguments(int dtype, int kv_dtype, int hq, int hkv, int d, const void *k_pages, const void *v_pages, int64_t page_stride,
+                             int64_t head_stride, int64_t slot_stride, int pages, int page_size, const int32_t *starts, const int32_t *lens,
+                             const int32_t *table, int cols, int seqs, int tokens, PagedKv *kv, PagedRows *rows);
+// The GPU of `dev` is the calling thread's current one while this lives.
+struct PagedGpu {
+    int before = -1;
+    fh_status enter(const fh_device *dev);
+    ~PagedGpu();
+};

@@ -15,7 +15,7 @@ import numpy as np
 from . import _lib
 from ._lib import (F16, F32, MASK_ADDITIVE, MASK_CAUSAL, MASK_NONE, Q4_0, Q4_K, Q6_K, Q8_0, FusorHipError, check)
 
-__all__ = ["Device", "Tensor", "QMatrix", "RopeCache", "KvCache", "MaskKind", "GgmlType", "FusorHipError",
+__all__ = ["Device", "Tensor", "QMatrix", "RopeCache", "KvCache", "PagedKvCache", "PagedBatch", "MaskKind", "GgmlType", "FusorHipError",
            "GpuStandardSamplerParams", "GpuMirostat2SamplerParams", "GpuMirostat2Sampler"]
 
 
@@ -68,6 +68,7 @@ class MaskKind:
     QKMask, Causal, BatchKeyMask = MASK_ADDITIVE, MASK_CAUSAL, 3
 
 
+_ELEMENTS = {"f32": F32, "f16": F16, "bf16": _lib.DECODER_BF16}
 _NP = {"f32": np.float32, "f16": np.float16, "bf16": np.uint16, "u32": np.uint32, "i32": np.int32, "u8": np.uint8}
 
 
@@ -354,6 +355,25 @@ class Tensor:
             C.c_void_p(k.ptr), C.c_void_p(v.ptr), skv * d, d, hq, hkv, d, scale, skv, C.c_void_p(out.ptr)))
         return out
 
+    def paged_attention(self, cache: "PagedKvCache", batch: "PagedBatch", scale: float, window: int = 0, layer: int = 0,
+                        strides: Optional[Sequence[int]] = None, out: Optional["Tensor"] = None) -> "Tensor":
+        """fh_paged_attention: self [tokens, hq, d] against the pages of `batch`'s sequences, causal, over the last `window`
+        positions where that is not 0.  `strides` = (row, head) element strides of a view (of a fused projection's rows,
+        say) whose logical shape is self.shape.  The keys and values of the rows themselves must have been appended."""
+        tokens, hq, d = self.shape
+        if tokens != batch.tokens or d != cache.head_dim:
+            raise FusorHipError(_lib.FH_ERR_INVALID, f"rows of shape {self.shape} do not match a batch of {batch.tokens} rows "
+                                                     f"and a cache of head_dim {cache.head_dim}")
+        if out is None:
+            out = Tensor(self.device, self.shape, self.dtype)
+        st, sh = strides or (hq * d, d)
+        L = self.device._lib
+        status = L.fh_paged_attention(self.device._h, _ELEMENTS[self.dtype], cache.code, self.ptr, st, sh, hq, cache.kv_heads, d,
+                                      scale, window, *cache.layer(layer), *batch.args, batch.max_new, batch.max_len, out.ptr)
+        if status:
+            check(status)
+        return out
+
     def silu_mul(self, up: "Tensor") -> "Tensor":
         """silu(self) * up (activations.rs:47-65, raw/attention_layer.rs:195)"""
         out = Tensor(self.device, self.shape, "f32")
@@ -548,6 +568,14 @@ class RopeCache:
     def forward_interleaved(self, q, k, start_pos, **kw):
         return self._fwd(q, k, start_pos, True, **kw)
 
+    def forward_paged(self, q: Optional[Tensor], k: Tensor, v: Tensor, cache: "PagedKvCache", batch: "PagedBatch",
+                      positions: Optional[Tensor] = None, sections: Optional[Sequence[int]] = None, interleaved: bool = False,
+                      layer: int = 0, strides: Optional[Sequence[int]] = None, out: Optional[Tensor] = None) -> Optional[Tensor]:
+        """fh_paged_rope_append: q [tokens, hq, d] and k [tokens, hkv, d] turned, k and v written to the pages; returns the
+        turned q.  Positions are those in the cache, or `positions` [axes, tokens] (i32): `sections` says how many pairs of a
+        head follow each axis.  `strides` = (row, head) element strides of q, k and v (views of a fused projection's rows)."""
+        return cache._append(self, q, k, v, batch, positions, sections, interleaved, layer, strides, out)
+
 
 class KvCache:
     """fusor::KvCache (fusor-ml/fusor/src/cache/kv_cache.rs:24-63) for `layers` layers at once."""
@@ -584,3 +612,92 @@ class KvCache:
                 self.device._lib.fh_kvcache_destroy(self._h)
         except Exception:
             pass
+
+
+class PagedBatch:
+    """Which rows of a call belong to which sequence, and the pages of every sequence: device tensors that the calls read
+    when they run, so a program (or a captured graph) fills in new lengths and pages between them.
+
+    lens [n] i32: positions of every sequence, its new rows among them.  table [n, columns] i32: its pages.  starts [n + 1]
+    i32: sequence i has the rows starts[i] .. starts[i + 1] - 1; None: one row each.  tokens: rows of the tensors.  max_new:
+    the most new rows of a sequence.  max_len: the longest of lens where the host knows it (0: no matter)."""
+
+    def __init__(self, lens: Tensor, table: Tensor, starts: Optional[Tensor] = None, tokens: Optional[int] = None,
+                 max_new: Optional[int] = None, max_len: int = 0):
+        n, cols = table.shape
+        for what, t, shape in (("lens", lens, (n,)), ("table", table, (n, cols)), ("starts", starts, (n + 1,))):
+            if t is not None and (t.dtype != "i32" or t.shape != shape):
+                raise FusorHipError(_lib.FH_ERR_INVALID, f"{what} is i32 {shape}, not {t.dtype} {t.shape}")
+        if starts is not None and tokens is None:
+            raise FusorHipError(_lib.FH_ERR_INVALID, "a batch with starts needs its number of rows")
+        self.lens, self.table, self.starts = lens, table, starts
+        self.tokens = n if tokens is None else int(tokens)
+        self.max_new = (1 if starts is None else self.tokens) if max_new is None else int(max_new)
+        self.max_len = int(max_len)
+        self.args = (None if starts is None else starts.ptr, lens.ptr, table.ptr, cols, n, self.tokens)
+
+
+class PagedKvCache:
+    """Keys and values of many sequences in pages, `layers` layers at once: k and v [layers, pages, kv_heads, page_size,
+    head_dim].  Which page holds what is the caller's: a PagedBatch names the pages of its sequences."""
+
+    def __init__(self, device: Device, layers: int, kv_heads: int, head_dim: int, pages: int, page_size: int, dtype: str = "f16"):
+        shape = (layers, pages, kv_heads, page_size, head_dim)
+        self._over(Tensor.zeros(device, shape, dtype), Tensor.zeros(device, shape, dtype))
+
+    @staticmethod
+    def over(k: Tensor, v: Tensor) -> "PagedKvCache":
+        """The same over tensors that the program has: [pages, kv_heads, page_size, head_dim], or a layer's each."""
+        c = PagedKvCache.__new__(PagedKvCache)
+        c._over(k, v)
+        return c
+
+    def _over(self, k: Tensor, v: Tensor) -> None:
+        shape = k.shape if len(k.shape) == 5 else (1, *k.shape)
+        if len(shape) != 5 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _ELEMENTS:
+            raise FusorHipError(_lib.FH_ERR_INVALID, f"pages of shapes {k.shape}, {v.shape} and types {k.dtype}, {v.dtype}")
+        self.device, self.k, self.v, self.dtype, self.code = k.device, k, v, k.dtype, _ELEMENTS[k.dtype]
+        self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = shape
+        row = self.page_size * self.head_dim
+        step = k.nbytes // self.layers
+        self._layers = [(k.ptr + i * step, v.ptr + i * step, self.kv_heads * row, row, self.head_dim, self.pages, self.page_size)
+                        for i in range(self.layers)]
+
+    def layer(self, layer: int):
+        """A layer's pointers, strides and sizes as the library takes them."""
+        if not 0 <= layer < self.layers:
+            raise FusorHipError(_lib.FH_ERR_INVALID, f"layer {layer} of {self.layers}")
+        return self._layers[layer]
+
+    def append(self, k: Tensor, v: Tensor, batch: PagedBatch, layer: int = 0, strides: Optional[Sequence[int]] = None) -> None:
+        """k, v [tokens, kv_heads, head_dim] written to their pages as they are."""
+        self._append(None, None, k, v, batch, None, None, False, layer, strides, None)
+
+    def _append(self, rope, q, k, v, batch, positions, sections, interleaved, layer, strides, out):
+        n, hkv, d = k.shape
+        if k.shape != v.shape or k.dtype != v.dtype or n != batch.tokens or hkv != self.kv_heads or d != self.head_dim:
+            raise FusorHipError(_lib.FH_ERR_INVALID, f"k {k.shape} and v {v.shape} do not match a batch of {batch.tokens} rows and a "
+                                                     f"cache of {self.kv_heads} heads of {self.head_dim}")
+        hq = hkv
+        if q is not None:
+            hq = q.shape[1]
+            if q.shape != (n, hq, d) or q.dtype != k.dtype:
+                raise FusorHipError(_lib.FH_ERR_INVALID, f"q {q.shape} {q.dtype} does not match k {k.shape} {k.dtype}")
+            if out is None:
+                out = Tensor(self.device, q.shape, q.dtype)
+        cos, sin, rows, pairs, axes, sec = None, None, 0, 0, 1, None
+        if rope is not None:
+            cos, sin, (rows, pairs) = rope.cos.ptr, rope.sin.ptr, rope.cos.shape
+            if sections is not None:
+                axes, sec = len(sections), (C.c_int32 * len(sections))(*sections)
+            if positions is not None and (positions.dtype != "i32" or positions.shape != (axes, n)):
+                raise FusorHipError(_lib.FH_ERR_INVALID, f"positions are i32 {(axes, n)}, not {positions.dtype} {positions.shape}")
+        st, sh = strides or (0, d)
+        L = self.device._lib
+        status = L.fh_paged_rope_append(self.device._h, _ELEMENTS[k.dtype], self.code, None if q is None else q.ptr, st or hq * d, sh,
+                                        k.ptr, v.ptr, st or hkv * d, sh, hq, hkv, d, cos, sin, rows, pairs,
+                                        None if positions is None else positions.ptr, sec, axes, int(interleaved), *self.layer(layer),
+                                        *batch.args, None if q is None else out.ptr)
+        if status:
+            check(status)
+        return out if q is not None else None

@@ -1,0 +1,234 @@
+"""Attention over a paged cache against the definition in 64 bits: one new token a sequence (split over the cache and joined)
+and several (tiles of a prompt); slots that nothing may see hold NaN in every case."""
+import numpy as np
+import pytest
+
+from pagedgen import Pages, near, unpack
+from kalosm_amd.fusor import FusorHipError, PagedBatch, Tensor
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "f16"), ("f32", "bf16")]
+
+
+def run(dev, p, window=0, q=None, scale=None, **kw):
+    cache, batch = p.put(dev)
+    for name, value in kw.items():
+        setattr(batch, name, value)
+    qt = Tensor.from_slice(dev, p.q, p.act) if q is None else q
+    out = Tensor.filled_bytes(dev, (p.tokens, p.hq, p.d), 0xFF, p.act)  # NaN where nothing is written
+    qt.paged_attention(cache, batch, scale or p.d ** -0.5, window=window, out=out)
+    return unpack(out.as_slice(), p.act)
+
+
+def check(dev, p, window=0, what="", scale=None, **kw):
+    got = run(dev, p, window, scale=scale, **kw)
+    want, bound = p.attention(scale or p.d ** -0.5, window)
+    lo, hi = int(p.starts[0]), int(p.starts[-1])
+    near(got[lo:hi], want[lo:hi], bound[lo:hi], what)
+    assert np.isnan(got[:lo]).all() and np.isnan(got[hi:]).all(), f"{what}: rows of no sequence were written"
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (5, 1, 64), (4, 4, 96), (16, 1, 128), (3, 3, 8), (40, 2, 256), (6, 2, 200), (18, 1, 72)])
+def test_step_heads(dev, act, kept, hq, hkv, d):
+    lens = [1, 2, 15, 16, 17, 31, 33, 300]
+    check(dev, Pages(hq + d, [1] * len(lens), lens, hq, hkv, d, 16, act, kept), what=f"{act}/{kept} {hq}/{hkv} of {d}")
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+@pytest.mark.parametrize("page", [16, 32, 64, 256, 4096])
+def test_step_pages(dev, act, kept, page):
+    lens = [page - 1, page, page + 1, 2 * page + 5, 1]
+    check(dev, Pages(page, [1] * len(lens), lens, 8, 2, 64, page, act, kept), what=f"{act}/{kept} pages of {page}")
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+@pytest.mark.parametrize("lens", [[4097], [20011], [5000, 1, 0, 700, 2048, 64, 9, 6001]])
+def test_step_long(dev, act, kept, lens):
+    check(dev, Pages(len(lens), [1] * len(lens), lens, 8, 2, 128, 64, act, kept), what=f"{act}/{kept} {lens}")
+
+
+def test_step_many_sequences(dev):
+    rng = np.random.default_rng(5)
+    lens = [int(x) for x in rng.integers(0, 90, 333)]
+    check(dev, Pages(9, [1] * len(lens), lens, 4, 2, 64, 16, "f16", "f16"), what="333 short sequences")
+    check(dev, Pages(9, [1] * len(lens), lens, 4, 4, 128, 32, "bf16", "bf16"), what="333 short sequences, a head each")
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [7, 1, 33]])
+@pytest.mark.parametrize("window", [1, 16, 37, 1000])
+@pytest.mark.parametrize("act,kept", [("f16", "f16"), ("f32", "f32"), ("bf16", "bf16")])
+def test_window(dev, new, window, act, kept):
+    check(dev, Pages(window, new, [777, 1, 130], 8, 2, 64, 16, act, kept), window, what=f"window {window}, rows {new}")
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 3, 130]])
+@pytest.mark.parametrize("act,kept", [("f16", "f16"), ("f32", "f32"), ("f32", "bf16")])
+def test_holes(dev, new, act, kept):
+    """Entries that are no page are not seen: below 0, past the pool, in the middle of a sequence, all of one."""
+    p = Pages(3, new, [700, 65, 130], 8, 2, 128, 16, act, kept)
+    p.table[0, 3], p.table[0, 17], p.table[0, 30:33] = -1, p.pages, (2 ** 31 - 1, -2 ** 31, p.pages + 7)
+    p.table[1, :] = -5
+    p.table[2, 0] = -1
+    check(dev, p, what=f"holes, rows {new}")
+    check(dev, p, 64, what=f"holes and a window, rows {new}")
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (5, 1, 64), (4, 4, 96), (7, 1, 128), (3, 3, 8), (2, 1, 256), (6, 2, 200)])
+def test_prompt_heads(dev, act, kept, hq, hkv, d):
+    p = Pages(hq + d, [70, 2, 129, 1, 31], [70, 90, 140, 1, 300], hq, hkv, d, 16, act, kept)
+    check(dev, p, what=f"{act}/{kept} {hq}/{hkv} of {d}")
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+@pytest.mark.parametrize("new,lens", [([2], [2]), ([64], [64]), ([65], [65]), ([128], [129]), ([300], [300]), ([5], [3000]), ([257, 255], [257, 1200])])
+def test_prompt_lengths(dev, act, kept, new, lens):
+    check(dev, Pages(sum(lens), new, lens, 4, 1, 128, 32, act, kept), what=f"{act}/{kept} {new} of {lens}")
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 256, 4096])
+@pytest.mark.parametrize("act,kept", [("f16", "f16"), ("f32", "f32")])
+def test_prompt_pages(dev, page, act, kept):
+    check(dev, Pages(page, [100, 3], [page + 37, 2 * page - 1], 4, 2, 64, page, act, kept), what=f"pages of {page}")
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [5, 0, 40]])
+@pytest.mark.parametrize("act,kept", [("f16", "f16"), ("f32", "f32"), ("f32", "f16"), ("bf16", "bf16")])
+def test_slot_major_pages_and_rows_of_no_sequence(dev, new, act, kept):
+    p = Pages(11, new, [200, 17, 90], 6, 3, 64, 16, act, kept, slot_major=True, before=3, behind=4)
+    check(dev, p, what="pages [page][slot][head]")
+
+
+@pytest.mark.parametrize("new", [[1, 1], [20, 130]])
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+def test_rows_of_a_fused_projection(dev, new, act):
+    """q is a view: other strides, and an odd beginning."""
+    p = Pages(12, new, [150, 333], 4, 2, 128, 16, act, act)
+    wide = np.zeros((p.tokens, 8 * 128 + 1), p.q.dtype)
+    wide[:, 1:513] = p.q.reshape(p.tokens, 512)
+    t = Tensor.from_slice(dev, wide.reshape(-1), act)
+    view = Tensor(dev, p.q.shape, act, ptr=t.ptr + wide.itemsize)
+    cache, batch = p.put(dev)
+    out = view.paged_attention(cache, batch, 128 ** -0.5, strides=(8 * 128 + 1, 128))
+    want, bound = p.attention(128 ** -0.5)
+    near(unpack(out.as_slice(), act), want, bound, f"a view of {act}")
+
+
+@pytest.mark.parametrize("new", [[1, 1], [50, 3]])
+@pytest.mark.parametrize("act,kept", TYPES)
+def test_sharp_and_large_values(dev, new, act, kept):
+    """Scores far apart, and values next to the ends of the types' ranges."""
+    p = Pages(21, new, [900, 70], 4, 2, 64, 16, act, kept, spread=30.0)
+    check(dev, p, what="scores of some hundreds")
+    p.v = np.where(np.isnan(unpack(p.v, kept)), p.v, {"f16": lambda a: (a * np.float16(2 ** -14)), "f32": lambda a: a * np.float32(1e30), "bf16": lambda a: a}[kept](p.v)).astype(p.v.dtype)
+    check(dev, p, what="values of another size")
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+def test_infinite_and_nan_rows_stay_theirs(dev, act, kept):
+    """An infinity or a NaN in V reaches the rows that see it, and no others; -inf in K takes its position out."""
+    for new in ([1, 1, 1], [90, 1, 70]):
+        p = Pages(31, new, [90, 200, 300], 4, 2, 64, 16, act, kept)
+        inf = {"f32": np.float32(np.inf), "f16": np.float16(np.inf), "bf16": np.uint16(0x7F80)}[kept]
+        nan = {"f32": np.float32(np.nan), "f16": np.float16(np.nan), "bf16": np.uint16(0x7FC0)}[kept]
+
+        def at(a, i, pos):
+            return a[p.table[i, pos // 16], :, pos % 16]
+
+        at(p.v, 0, 89)[:, 5] = nan   # only the last row of the first sequence sees it
+        at(p.v, 2, 290)[:, 7] = inf
+        got = run(dev, p)
+        with np.errstate(invalid="ignore"):
+            want, bound = p.attention(64 ** -0.5)
+        fine = np.isfinite(want)
+        assert (np.isfinite(got) == fine).all(), f"{new}: {np.argwhere(np.isfinite(got) != fine)[:5].tolist()}"
+        near(np.where(fine, got, 0), np.where(fine, want, 0), np.where(fine, bound, 1), f"{act}/{kept} {new}")
+
+
+@pytest.mark.parametrize("new", [[1] * 5, [40, 3, 1, 0, 65]])
+def test_max_len_only_chooses(dev, new):
+    p = Pages(41, new, [900, 3, 4100, 64, 65], 8, 2, 128, 32, "f16", "f16")
+    want, bound = p.attention(128 ** -0.5)
+    for n in (0, 1, 100, 4100, 1 << 20):
+        got = run(dev, p, max_len=n)
+        near(got, want, bound, f"max_len {n}")
+
+
+def test_one_row_each_without_starts(dev):
+    p = Pages(51, [1, 1, 1], [10, 500, 77], 4, 2, 64, 16, "f16", "f16")
+    cache, batch = p.put(dev)
+    alone = PagedBatch(batch.lens, batch.table)
+    q = Tensor.from_slice(dev, p.q, "f16")
+    a, b = (q.paged_attention(cache, x, 0.125).as_slice() for x in (batch, alone))
+    assert np.array_equal(a.view(np.uint16), b.view(np.uint16))
+
+
+def test_lengths_that_do_not_fit_are_safe(dev):
+    """Lengths past the table, below the new rows and below 0; starts past the rows."""
+    p = Pages(61, [1, 4, 2], [40, 60, 30], 4, 2, 64, 16, "f16", "f16")
+    cache, batch = p.put(dev)
+    q = Tensor.from_slice(dev, p.q, "f16")
+    want, bound = p.attention(0.125)
+    for lens in ([2 ** 31 - 1, 60, -7], [10 ** 6, 2, 0]):
+        b = PagedBatch(Tensor.from_slice(dev, np.array(lens, np.int32), "i32"), batch.table, batch.starts, tokens=p.tokens, max_new=4)
+        got = unpack(q.paged_attention(cache, b, 0.125).as_slice(), "f16")
+        if lens[1] == 60:
+            near(got[1:5], want[1:5], bound[1:5], "the others")
+        else:
+            assert (got[1:3] == 0).all()  # positions below 0 see nothing
+        assert (got[5:] == 0).all()
+    starts = Tensor.from_slice(dev, np.array([-4, 1, 5, 100], np.int32), "i32")
+    b = PagedBatch(batch.lens, batch.table, starts, tokens=p.tokens, max_new=50)
+    near(unpack(q.paged_attention(cache, b, 0.125).as_slice(), "f16")[1:5], want[1:5], bound[1:5], "rows of the middle sequence")
+
+
+def test_graphs_share_their_scratch(dev):
+    """Two captured calls and an eager one in between, replayed in turn with lengths that change."""
+    a = Pages(71, [1, 1], [3000, 400], 8, 2, 128, 32, "f16", "f16")
+    b = Pages(72, [50], [5000], 8, 2, 128, 32, "bf16", "bf16")
+    made = []
+    for p in (a, b):
+        cache, batch = p.put(dev)
+        q, out = Tensor.from_slice(dev, p.q, p.act), Tensor.zeros(dev, p.q.shape, p.act)
+        q.paged_attention(cache, batch, 128 ** -0.5, out=out)
+        made.append((p, cache, batch, q, out))
+    graphs = []
+    for p, cache, batch, q, out in made:
+        dev.graph_begin()
+        q.paged_attention(cache, batch, 128 ** -0.5, out=out)
+        graphs.append(dev.graph_end())
+    for turn in range(3):
+        for (p, cache, batch, q, out), graph in zip(made, graphs):
+            p.lens = [x - 37 * turn for x in p.lens]
+            t = np.array(p.lens, np.int32)
+            from kalosm_amd import _lib
+            _lib.check(dev._lib.fh_upload(dev._h, batch.lens.ptr, t.ctypes.data, t.nbytes))
+            graph.launch()
+            want, bound = p.attention(128 ** -0.5)
+            near(unpack(out.as_slice(), p.act), want, bound, f"replay {turn}")
+            q.paged_attention(cache, batch, 128 ** -0.5, out=out)
+            near(unpack(out.as_slice(), p.act), want, bound, f"eager {turn}")
+            p.lens = [x + 37 * turn for x in p.lens]
+
+
+def test_same_call_same_bits(dev):
+    for new in ([1] * 9, [33] * 9):
+        p = Pages(81, new, [100 * i + 40 for i in range(9)], 8, 2, 128, 16, "f32", "f16")
+        first = run(dev, p)
+        for _ in range(3):
+            assert np.array_equal(run(dev, p), first)
+
+
+def test_refused(dev):
+    p = Pages(91, [1], [20], 4, 2, 64, 16, "f16", "f16")
+    cache, batch = p.put(dev)
+    with pytest.raises(FusorHipError, match="match a batch"):
+        Tensor.zeros(dev, (2, 4, 64), "f16").paged_attention(cache, batch, 0.1)
+    with pytest.raises(FusorHipError, match="rows of type"):
+        Tensor.zeros(dev, (1, 4, 64), "bf16").paged_attention(cache, batch, 0.1)
+    with pytest.raises(FusorHipError, match="share"):
+        Tensor.zeros(dev, (1, 3, 64), "f16").paged_attention(cache, batch, 0.1)
+    with pytest.raises(FusorHipError, match="layer 1"):
+        Tensor.zeros(dev, (1, 4, 64), "f16").paged_attention(cache, batch, 0.1, layer=1)
