@@ -21,10 +21,8 @@ struct PagedSeq {
     int first;     // position of the first of them (below 0 where the sequence is said to be shorter than its new rows)
     int len;       // positions that can be read: no further than the table's row reaches
 };
-__device__ __forceinline__ PagedSeq paged_seq(const PagedRows &r, int shift, int i) {
+__device__ __forceinline__ PagedSeq paged_seq(const PagedRows &r, int shift, int len, int from, int to) {
     PagedSeq s;
-    int len = r.lens[i], from = i, to = i + 1;
-    if (r.starts) from = r.starts[i], to = r.starts[i + 1];
     len = len < 0 ? 0 : len > FH_PAGED_MAX ? FH_PAGED_MAX : len;
     from = from < 0 ? 0 : from > r.tokens ? r.tokens : from;
     to = to < from ? from : to > r.tokens ? r.tokens : to;
@@ -35,11 +33,32 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedRows &r, int shift, int
     s.len = len < reach ? len : (int)reach;
     return s;
 }
+__device__ __forceinline__ PagedSeq paged_seq(const PagedRows &r, int shift, int i) {
+    return r.starts ? paged_seq(r, shift, r.lens[i], r.starts[i], r.starts[i + 1]) : paged_seq(r, shift, r.lens[i], i, i + 1);
+}
+// The same for an index that is the wavefront's, by scalar loads: their waits leave the vector loads that are on their way alone.
+typedef const __attribute__((address_space(4))) int *PagedScalars;
+__device__ __forceinline__ int paged_scalar(const int *p, int64_t i) { return ((PagedScalars)(uintptr_t)p)[i]; }
+__device__ __forceinline__ PagedSeq paged_seq_scalar(const PagedRows &r, int shift, int i) {
+    const int len = paged_scalar(r.lens, i);
+    return r.starts ? paged_seq(r, shift, len, paged_scalar(r.starts, i), paged_scalar(r.starts, i + 1)) : paged_seq(r, shift, len, i, i + 1);
+}
 
 // Arguments both entry points check, without touching a device: FH_OK, or an error with its message.  `kv` and `rows` are filled in.
 fh_status fh_paged_arguments(int dtype, int kv_dtype, int hq, int hkv, int d, const void *k_pages, const void *v_pages, int64_t page_stride,
                              int64_t head_stride, int64_t slot_stride, int pages, int page_size, const int32_t *starts, const int32_t *lens,
                              const int32_t *table, int cols, int seqs, int tokens, PagedKv *kv, PagedRows *rows);
+// Arguments of fh_paged_attention that its kernels share.
+struct PagedCall {
+    const void *q;
+    void *out;
+    int64_t q_st, q_sh; // elements
+    PagedKv kv;
+    PagedRows rows;
+    float scale;
+    int window, hq, hkv, d;
+};
+fh_status fh_paged_step(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len); // rows.max_new = 1
 // The GPU of `dev` is the calling thread's current one while this lives.
 struct PagedGpu {
     int before = -1;

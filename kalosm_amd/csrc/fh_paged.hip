@@ -234,13 +234,15 @@ extern "C" fh_status fh_paged_attention(fh_device *dev, int32_t dtype, int32_t k
     FH_TRY(fh_paged_arguments(dtype, kv_dtype, hq, hkv, d, k_pages_dev, v_pages_dev, page_stride, head_stride, slot_stride, pages, page_size,
                               starts_dev, lens_dev, table_dev, table_cols, seqs, tokens, &kv, &rows));
     FH_REQUIRE(q_dev && out_dev, "NULL argument");
-    FH_REQUIRE(scale > 0.f && scale < INFINITY, "scale %g", (double)scale);
+    FH_REQUIRE(scale >= 0x1p-60f && scale < INFINITY, "scale %g", (double)scale);
     FH_REQUIRE(window >= 0 && max_new >= 0 && max_len >= 0, "window %d, max_new %d, max_len %d", window, max_new, max_len);
     FH_REQUIRE(dev, "NULL device");
     if (!tokens || !seqs || !max_new) return FH_OK;
     rows.max_new = max_new < tokens ? max_new : tokens;
     PagedGpu gpu;
     FH_TRY(gpu.enter(dev));
+    const PagedCall call = {q_dev, out_dev, q_st, q_sh, kv, rows, scale, window, hq, hkv, d};
+    if (rows.max_new == 1) return fh_paged_step(dev, dtype, kv_dtype, call, max_len);
 #define FH_PR(TX, TP)                                                                                                                              \
     k_paged_rows<TX, TP><<<dim3((unsigned)hq, (unsigned)rows.max_new, (unsigned)seqs), dim3(64), 0, dev->stream>>>((const TX *)q_dev, q_st, q_sh, hq, hkv, d, scale,   \
                                                                                                           window, kv, rows, (TX *)out_dev)

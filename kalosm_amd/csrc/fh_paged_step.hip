@@ -1,0 +1,523 @@
+// Attention of one new token of every sequence over its pages: softmax(scale q . K^T) . V for the query heads that share a KV
+// head, every key and value read once.
+//
+// What it has to do is a stream of cache rows: 4 d flops a query head and key against 4 d bytes a KV head and key (16-bit
+// pages), so the arithmetic goes to the matrix cores and has to stay out of the loads' way.  A wavefront takes tiles of 32
+// positions (f32 pages: 16), 8 KB of K and 8 KB of V at head_dim 128, straight into registers; nothing goes through LDS.
+//   scores  S^T (keys x heads) = K . Q^T    A: K rows as they were loaded (lane (n, g): key n of 16, values 8 g ..), B: Q^T
+//   output  O^T (d x heads)   += V^T . P^T  B: the scores' accumulators, exponentiated, as they sit in the registers: slot (g, j)
+//           of the product is key 4 g + j of the tile's first half (j < 4) or second.  A lane loads 16 bytes of the eight rows of
+//           its slots, d = 8 n ..; operand e takes element e of each of them - row n of that product is d = 8 n + e - so the
+//           transposition of V is 32 byte permutations a tile and no exchange between lanes.  A lane ends up with one head's
+//           outputs d = 32 g .. 32 g + 31.
+// Both halves of a tile (16 positions) lie in one page each: a page's address is scalar, a lane's offset within it constant.
+// f32 pages use v_mfma_f32_16x16x4_f32 the same way, in full f32.  f32 rows over 16-bit pages: Q and P are taken as sums of
+// 16-bit terms, two of f16 (22 bits; Q's rows brought to 2^14 first), three of bf16 (24 bits).  Weights of bf16 rows have two
+// terms, which cost nothing here, weights of f16 rows one, 2^14 times what they are, so that those below 2^-24 of the largest count.
+//
+// The tiles of all (sequence, KV head) pairs are one line, cut into equal stretches, one a workgroup, whatever the lengths: a
+// workgroup has the end of one pair, whole pairs, and the beginning of another.  Its wavefronts take a pair's tiles in turn,
+// each with its own running maximum and sum, and are joined through LDS where the pair (or the stretch) ends.  What is not a
+// whole pair goes to scratch memory, two places a workgroup, and whoever of the pair's workgroups counts itself in last adds
+// them up, in their order: the same bits in every run.  Pairs of few tiles are a workgroup each, and nothing is joined.
+#include "fh_paged.h"
+#include <type_traits>
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float ps_rows_max(float a) { // over the four 16-lane rows of the wavefront
+    const uint32_t u = __float_as_uint(a);
+    auto s16 = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    a = fmaxf(__uint_as_float(s16[0]), __uint_as_float(s16[1]));
+    const uint32_t w = __float_as_uint(a);
+    auto s32 = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return fmaxf(__uint_as_float(s32[0]), __uint_as_float(s32[1]));
+}
+__device__ __forceinline__ float ps_rows_sum(float a) {
+    const uint32_t u = __float_as_uint(a);
+    auto s16 = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    a = __uint_as_float(s16[0]) + __uint_as_float(s16[1]);
+    const uint32_t w = __float_as_uint(a);
+    auto s32 = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return __uint_as_float(s32[0]) + __uint_as_float(s32[1]);
+}
+__device__ __forceinline__ floatx4 ps_mfma(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ floatx4 ps_mfma(bf8 a, bf8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ int ps_uniform(int a) { return __builtin_amdgcn_readfirstlane(a); }
+
+template <typename TP> struct PsVec { typedef half8 type; };
+template <> struct PsVec<fh_bf> { typedef bf8 type; };
+
+struct PsArgs {
+    PagedCall c;
+    int blocks; // of up to 16 query heads a KV head
+    int whole;  // a pair a workgroup
+    int least;  // tiles a stretch has at least
+    int place;  // floats of a part
+    float *part;
+    uint32_t *arrived;
+};
+
+// A pair's tiles: positions first * TK .. (first + tiles) * TK - 1, of which begin .. end - 1 are seen.
+struct PsSpan {
+    int row, begin, end, first, tiles;
+};
+template <int TK> __device__ __forceinline__ PsSpan ps_span(const PagedSeq &s, int window) {
+    PsSpan r;
+    r.row = s.row;
+    const int p = s.first;
+    r.end = p + 1 < s.len ? p + 1 : s.len;
+    r.end = r.end < 0 ? 0 : r.end;
+    r.begin = window && p - window + 1 > 0 ? p - window + 1 : 0;
+    r.begin = r.begin < r.end ? r.begin : r.end;
+    r.first = r.begin / TK;
+    r.tiles = (r.end + TK - 1) / TK - r.first;
+    r.tiles = s.rows < 1 ? 0 : r.tiles < 1 ? 1 : r.tiles; // (a row that sees nothing has one tile, all masked: it writes zeros)
+    return r;
+}
+
+template <typename TX, typename TP, int DP, int NWV>
+__global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
+    constexpr bool F32 = sizeof(TP) == 4, F16 = __is_same(TP, fh_half), MIXED = sizeof(TX) != sizeof(TP);
+    constexpr int TK = F32 ? 16 : 32, HALVES = TK / 16;
+    constexpr int QT = F32 ? 1 : !MIXED ? 1 : F16 ? 2 : 3, PT = F32 ? 1 : MIXED ? (F16 ? 2 : 3) : F16 ? 1 : 2; // terms
+    constexpr int KL = DP * (int)sizeof(TP) / 64;                     // 16-byte pieces of a row of K in a lane
+    constexpr int VB = DP * (int)sizeof(TP) / 16 < 16 ? 8 : 16, VL = DP * (int)sizeof(TP) / 16 / VB; // pieces of a row of V: their bytes, and how many
+    constexpr int VE = VB / (int)sizeof(TP), NA = VL * VE;            // values of a piece; output tiles: d = 16 VE c + VE (4 g + i) + e
+    constexpr int THREADS = 64 * NWV;
+    typedef typename PsVec<TP>::type vec8;
+    extern __shared__ __attribute__((aligned(16))) float ps_lds[];
+    __shared__ float s_st[NWV * 16 * 2];
+    __shared__ uint32_t s_last;
+    const int tid = threadIdx.x, wave = ps_uniform(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const PagedKv &kv = a.c.kv;
+    const PagedRows &rows = a.c.rows;
+    const int group = a.c.hq / a.c.hkv, H = a.c.hkv * a.blocks, page_mask = (1 << kv.shift) - 1;
+
+    // ---- this workgroup's stretch of the line: tiles lo .. hi - 1; its first pair is of sequence b, which begins at `at`
+    int64_t step = 0, lo = 0, hi = 0, at = 0;
+    int b = 0;
+    if (a.whole) b = ps_uniform((int)blockIdx.x / H);
+    else {
+        auto tiles_of = [&](int i) { return i < rows.seqs ? ps_span<TK>(paged_seq(rows, kv.shift, i), a.c.window).tiles : 0; };
+        auto scan = [&](int64_t x) { // inclusive, over the lanes
+#pragma unroll
+            for (int w = 1; w < 64; w *= 2) {
+                const int64_t y = __shfl_up(x, w);
+                if (lane >= w) x += y;
+            }
+            return x;
+        };
+        auto uniform = [](int64_t x) { return (int64_t)((uint64_t)(uint32_t)ps_uniform((int)(x >> 32)) << 32 | (uint32_t)ps_uniform((int)x)); };
+        int64_t sums = scan(tiles_of(lane)), total = __shfl(sums, 63);
+        for (int c = 64; c < rows.seqs; c += 64) {
+            int64_t x = tiles_of(c + lane);
+#pragma unroll
+            for (int w = 32; w; w >>= 1) x += __shfl_xor(x, w);
+            total += x;
+        }
+        total = uniform(total) * H;
+        step = (total + gridDim.x - 1) / gridDim.x;
+        step = step < a.least ? a.least : step;
+        lo = step * blockIdx.x, hi = lo + step < total ? lo + step : total;
+        if (lo >= total) return;
+        int64_t before = 0;
+        int c = 0;
+        for (;; c += 64) { // (lo < total: it ends)
+            if (c) sums = scan(tiles_of(c + lane));
+            const int64_t here = uniform(__shfl(sums, 63));
+            if ((before + here) * H > lo) break;
+            before += here;
+        }
+        const int in = __popcll(__ballot((before + sums) * H <= lo)); // sequences of these 64 that end before
+        b = ps_uniform(c + in);
+        at = uniform(before + (in ? __shfl(sums, in - 1) : 0)) * H;
+    }
+
+    // ---- a pair on the line: sequence b, block hh of its query heads
+    struct Cursor {
+        PsSpan s;
+        int b, hh, kh, from, to; // tiles from .. to - 1 of the pair lie in the stretch
+        int64_t pair_at;     // where the pair begins on the line
+    };
+    auto enter = [&](Cursor &c) { // the part of the pair that lies in the stretch
+        const int64_t f = lo - c.pair_at, e = hi - c.pair_at;
+        c.from = f > 0 ? (int)f : 0;
+        c.to = e < c.s.tiles ? (int)e : c.s.tiles;
+        c.kh = a.blocks == 1 ? c.hh : c.hh / a.blocks;
+    };
+    auto next_pair = [&](Cursor &c) { // false at the stretch's end
+        c.pair_at += c.s.tiles;
+        if (c.pair_at >= hi) return false;
+        if (++c.hh == H) {
+            c.hh = 0;
+            do c.s = ps_span<TK>(paged_seq_scalar(rows, kv.shift, ++c.b), a.c.window);
+            while (c.s.tiles == 0); // (the line goes on, so there is one)
+        }
+        enter(c);
+        return true;
+    };
+    Cursor cur;
+    cur.b = b;
+    cur.s = ps_span<TK>(paged_seq_scalar(rows, kv.shift, b), a.c.window);
+    if (a.whole) {
+        if (cur.s.tiles == 0) return;
+        cur.hh = (int)blockIdx.x % H;
+        cur.pair_at = 0, hi = cur.s.tiles;
+    } else {
+        cur.hh = (int)((lo - at) / cur.s.tiles);
+        cur.pair_at = at + (int64_t)cur.hh * cur.s.tiles;
+    }
+    enter(cur);
+
+    // ---- requests.  `ahead` is two tiles ahead of the products: the pages of its tile are asked for while the tile before is requested.
+    u32x4 kr[HALVES][KL];
+    typedef typename std::conditional<VB == 16, u32x4, u32x2>::type vpiece;
+    vpiece vr[HALVES][4][VL]; // [half][row 4 g + j][piece]
+    uint32_t k_off[KL], v_off[4], v_piece[VL];
+    {
+        const uint32_t slot = (uint32_t)kv.slot, row_bytes = (uint32_t)a.c.d * sizeof(TP);
+#pragma unroll
+        for (int s = 0; s < KL; s++) { // pieces behind the head's end: its first one again (Q is zero there)
+            const uint32_t piece = 64 * s + 16 * g;
+            k_off[s] = n * slot + (piece < row_bytes ? piece : 0);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) v_off[j] = (4 * g + j) * slot;
+#pragma unroll
+        for (int c = 0; c < VL; c++) {
+            const uint32_t piece = 16 * VB * c + VB * n;
+            v_piece[c] = piece < row_bytes ? piece : 0; // (outputs that are not stored)
+        }
+    }
+    Cursor ahead = cur;
+    int t = cur.from + wave; // tile of `ahead`
+    bool more = true;
+    int next_key = 0, next_kh = 0, next_page[HALVES]; // the tile whose pages have been asked for
+    const char *kb[HALVES], *vb[HALVES];              // the tile that is requested,
+    int key0 = 0;                                     // its first position
+    uint32_t holes = 0;                               // and its halves without a page
+    auto look_up = [&]() {
+        while (more && t >= ahead.to) {
+            more = next_pair(ahead);
+            if (more) t = ahead.from + wave;
+        }
+        next_key = more ? (ahead.s.first + t) * TK : 0; // (behind the end: something that is there, and dropped)
+        next_kh = ahead.kh;
+#pragma unroll
+        for (int h = 0; h < HALVES; h++) {
+            const int col = (next_key + 16 * h) >> kv.shift;
+            next_page[h] = paged_scalar(rows.table, (int64_t)ahead.b * rows.cols + (col < rows.cols ? col : rows.cols - 1));
+        }
+        t += NWV;
+    };
+    auto place = [&]() {
+        key0 = next_key, holes = 0;
+#pragma unroll
+        for (int h = 0; h < HALVES; h++) {
+            int page = next_page[h];
+            if ((unsigned)page >= (unsigned)kv.pages) page = 0, holes |= 1u << h;
+            const int64_t o = page * kv.page + next_kh * kv.head + ((key0 + 16 * h) & page_mask) * kv.slot;
+            kb[h] = kv.k + o, vb[h] = kv.v + o;
+        }
+    };
+    auto ask_k = [&]() {
+#pragma unroll
+        for (int h = 0; h < HALVES; h++)
+#pragma unroll
+            for (int s = 0; s < KL; s++) kr[h][s] = *(const u32x4 *)(kb[h] + k_off[s]);
+    };
+    auto ask_v = [&]() {
+#pragma unroll
+        for (int h = 0; h < HALVES; h++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int c = 0; c < VL; c++) vr[h][j][c] = *(const vpiece *)(vb[h] + (v_off[j] + v_piece[c]));
+    };
+    look_up();
+    place();
+    ask_k();
+    ask_v();
+    look_up();
+
+    // ---- pair after pair
+    bool go = true;
+    while (go) {
+        const int skip = (cur.hh - cur.kh * a.blocks) * 16, h0 = cur.kh * group + skip, heads = group - skip < 16 ? group - skip : 16; // h0: first query head
+        // Q^T operand: lane (head n, g), values as K's pieces have them; zeros for columns without a head and behind the head's end
+        vec8 qf[QT][F32 ? 1 : KL];
+        floatx4 qx[F32 ? KL : 1];
+        float sc2 = a.c.scale * 1.4426950408889634f; // scores in the log2 domain
+        {
+            const TX *qp = (const TX *)a.c.q + cur.s.row * a.c.q_st + (h0 + n) * a.c.q_sh;
+            constexpr int E = 16 / (int)sizeof(TP); // values of a piece
+            float x[KL][E], most = 0.f;
+#pragma unroll
+            for (int s = 0; s < KL; s++) {
+                const int dd = 4 * E * s + E * g;
+                TX v[E];
+#pragma unroll
+                for (int e = 0; e < E; e++) v[e] = (TX)0.f;
+                if (n < heads && dd < a.c.d) __builtin_memcpy(v, qp + dd, sizeof(v));
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    x[s][e] = (float)v[e];
+                    most = fmaxf(most, fabsf(x[s][e]));
+                }
+            }
+            if constexpr (MIXED && F16) { // brought to 2^14 .. 2^15
+                most = ps_rows_max(most);
+                int ex = 0;
+                if (most > 0.f && most < INFINITY) ex = 15 - __builtin_amdgcn_frexp_expf(most);
+                ex = ex < 60 ? ex : 60; // (below 2^-45 nothing is left to tell scores apart, and the scale must not vanish)
+                sc2 = ldexpf(sc2, -ex);
+#pragma unroll
+                for (int s = 0; s < KL; s++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) x[s][e] = ldexpf(x[s][e], ex);
+            }
+#pragma unroll
+            for (int s = 0; s < KL; s++) {
+                if constexpr (F32) qx[s] = floatx4{x[s][0], x[s][1], x[s][2], x[s][3]};
+                else
+#pragma unroll
+                    for (int u = 0; u < QT; u++)
+#pragma unroll
+                        for (int e = 0; e < E; e++) {
+                            const TP v = (TP)x[s][e];
+                            qf[u][s][e] = v;
+                            x[s][e] -= (float)v;
+                        }
+            }
+        }
+        float m_run = -INFINITY, l_run = 0.f;
+        floatx4 acc[NA];
+#pragma unroll
+        for (int e = 0; e < NA; e++) acc[e] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+        for (int u = cur.from + wave; u < cur.to; u += NWV) {
+            const int first = key0;
+            const uint32_t hole = holes;
+            floatx4 st[HALVES];
+#pragma unroll
+            for (int h = 0; h < HALVES; h++) {
+                st[h] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < KL; s++) {
+                    if constexpr (F32) {
+                        const floatx4 kx = __builtin_bit_cast(floatx4, kr[h][s]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) st[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[e], qx[s][e], st[h], 0, 0, 0);
+                    } else
+#pragma unroll
+                        for (int w = QT - 1; w >= 0; w--) st[h] = ps_mfma(__builtin_bit_cast(vec8, kr[h][s]), qf[w][s], st[h]);
+                }
+            }
+            place();
+            __builtin_amdgcn_sched_barrier(0);
+            ask_k();
+            look_up();
+            __builtin_amdgcn_sched_barrier(0);
+            // ---- positions that are not seen: scores -inf, values 0 (they may be anything)
+            const bool edge = first < cur.s.begin || first + TK > cur.s.end || hole;
+            if (edge) {
+#pragma unroll
+                for (int h = 0; h < HALVES; h++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int key = first + 16 * h + 4 * g + i;
+                        const bool seen = key >= cur.s.begin && key < cur.s.end && !(hole >> h & 1);
+                        st[h][i] = seen ? st[h][i] : -INFINITY;
+#pragma unroll
+                        for (int c = 0; c < VL; c++)
+#pragma unroll
+                            for (int w = 0; w < VB / 4; w++) vr[h][i][c][w] = seen ? vr[h][i][c][w] : 0u;
+                    }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < HALVES; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) mx = fmaxf(mx, st[h][i]);
+            mx = ps_rows_max(mx) * sc2;
+            const float m_new = fmaxf(m_run, mx);
+            const float ref = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = __builtin_amdgcn_exp2f(m_run - ref);
+            const float sub = F16 ? 14.f - ref : -ref;
+            float p[HALVES][4], ps = 0.f;
+#pragma unroll
+            for (int h = 0; h < HALVES; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    p[h][i] = __builtin_amdgcn_exp2f(fmaf(st[h][i], sc2, sub));
+                    ps += p[h][i];
+                }
+            l_run = l_run * alpha + ps; // of this lane's keys: the four rows of a column are added at the end
+            m_run = m_new;
+            if (__any(alpha != 1.f)) {
+#pragma unroll
+                for (int e = 0; e < NA; e++) acc[e] *= alpha;
+            }
+            if constexpr (F32) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int c = 0; c < VL; c++) {
+                        const floatx4 vx = __builtin_bit_cast(floatx4, vr[0][i][c]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[c * VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[e], p[0][i], acc[c * VE + e], 0, 0, 0);
+                    }
+            } else {
+                vec8 pb[PT];
+#pragma unroll
+                for (int w = 0; w < PT; w++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const TP x = (TP)p[j >> 2][j & 3];
+                        pb[w][j] = x;
+                        p[j >> 2][j & 3] -= (float)x;
+                    }
+#pragma unroll
+                for (int c = 0; c < VL; c++)
+#pragma unroll
+                    for (int e = 0; e < VE; e++) { // element e of the eight rows
+                        u32x4 x;
+                        const uint32_t pick = e & 1 ? 0x07060302u : 0x05040100u;
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            x[j] = __builtin_amdgcn_perm(vr[j >> 1][2 * (j & 1) + 1][c][e >> 1], vr[j >> 1][2 * (j & 1)][c][e >> 1], pick);
+#pragma unroll
+                        for (int w = PT - 1; w >= 0; w--) acc[c * VE + e] = ps_mfma(__builtin_bit_cast(vec8, x), pb[w], acc[c * VE + e]);
+                    }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            ask_v();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+
+        // ---- the wavefronts' results together: thread (head, four values)
+        l_run = ps_rows_sum(l_run);
+        if (n < heads) {
+            float *to = ps_lds + (wave * heads + n) * DP;
+#pragma unroll
+            for (int c = 0; c < VL; c++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int e = 0; e < VE; e += 4)
+                        *(floatx4 *)(to + 16 * VE * c + VE * (4 * g + i) + e) =
+                            floatx4{acc[c * VE + e][i], acc[c * VE + e + 1][i], acc[c * VE + e + 2][i], acc[c * VE + e + 3][i]};
+            if (g == 0) s_st[(wave * 16 + n) * 2] = m_run, s_st[(wave * 16 + n) * 2 + 1] = l_run;
+        }
+        __syncthreads();
+        const bool all = cur.from == 0 && cur.to == cur.s.tiles;
+        constexpr int PITCH = DP + 4; // of a part's head: values, maximum, sum
+        float *own = a.part + ((int64_t)blockIdx.x * 2 + (cur.from ? 0 : 1)) * a.place;
+        auto store = [&](int h, int dd, floatx4 x, float den) {
+            if (dd >= a.c.d) return;
+            const float inv = den == 0.f ? 0.f : 1.f / den;
+            TX y[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] = (TX)(x[i] * inv);
+            __builtin_memcpy((TX *)a.c.out + ((int64_t)cur.s.row * a.c.hq + h0 + h) * a.c.d + dd, y, sizeof(y));
+        };
+        for (int i = tid; i < heads * (DP / 4); i += THREADS) {
+            const int h = i / (DP / 4), dd = i % (DP / 4) * 4;
+            float mx = -INFINITY, den = 0.f;
+#pragma unroll
+            for (int w = 0; w < NWV; w++) mx = fmaxf(mx, s_st[(w * 16 + h) * 2]);
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < NWV; w++) {
+                const float f = __builtin_amdgcn_exp2f(s_st[(w * 16 + h) * 2] - ref);
+                x += *(const floatx4 *)(ps_lds + (w * heads + h) * DP + dd) * f;
+                den = fmaf(s_st[(w * 16 + h) * 2 + 1], f, den);
+            }
+            if (all) store(h, dd, x, den);
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) __hip_atomic_store(own + h * PITCH + dd + e, x[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (dd == 0) {
+                    __hip_atomic_store(own + h * PITCH + DP, mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    __hip_atomic_store(own + h * PITCH + DP + 1, den, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+            }
+        }
+        if (!all) {
+            const int w0 = (int)(cur.pair_at / step), parts = (int)((cur.pair_at + cur.s.tiles - 1) / step) - w0 + 1;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // written before this workgroup counts itself in
+            __syncthreads();
+            if (tid == 0) s_last = __hip_atomic_fetch_add(a.arrived + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (s_last == (uint32_t)parts - 1) {
+                if (tid == 0) __hip_atomic_store(a.arrived + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // as it was found
+                auto part = [&](int i) { return a.part + ((int64_t)(w0 + i) * 2 + (i ? 0 : 1)) * a.place; };
+                auto get = [&](const float *f) { return __hip_atomic_load(f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+                for (int i = tid; i < heads * (DP / 4); i += THREADS) {
+                    const int h = i / (DP / 4), dd = i % (DP / 4) * 4;
+                    float mx = -INFINITY, den = 0.f;
+                    for (int k = 0; k < parts; k++) mx = fmaxf(mx, get(part(k) + h * PITCH + DP));
+                    const float ref = mx == -INFINITY ? 0.f : mx;
+                    floatx4 x = {0.f, 0.f, 0.f, 0.f};
+                    for (int k = 0; k < parts; k++) {
+                        const float *f = part(k) + h * PITCH;
+                        const float w = __builtin_amdgcn_exp2f(get(f + DP) - ref);
+                        den = fmaf(get(f + DP + 1), w, den);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[e] = fmaf(get(f + dd + e), w, x[e]);
+                    }
+                    store(h, dd, x, den);
+                }
+            }
+        }
+        __syncthreads(); // the next pair's results go to the same places
+        go = next_pair(cur);
+    }
+}
+
+template <typename TX, typename TP, int DP, int NWV>
+static fh_status ps_launch(fh_device *dev, const PagedCall &call, int max_len) {
+    constexpr int TK = sizeof(TP) == 4 ? 16 : 32;
+    const int group = call.hq / call.hkv, heads = group < 16 ? group : 16;
+    PsArgs a = {};
+    a.c = call;
+    a.blocks = (group + 15) / 16;
+    a.place = heads * (DP + 4);
+    a.least = NWV;
+    int64_t longest = (int64_t)call.rows.cols << call.kv.shift;
+    if (max_len > 0 && max_len < longest) longest = max_len;
+    if (call.window > 0 && call.window + TK < longest) longest = call.window + TK;
+    const int64_t pairs = (int64_t)call.rows.seqs * call.hkv * a.blocks;
+    a.whole = longest <= 4 * NWV * TK;
+    unsigned grid = (unsigned)pairs;
+    if (!a.whole) {
+        grid = (unsigned)dev->compute_units;
+        FH_TRY(fh_dev_scratch(dev, (void **)&dev->part_buf, &dev->part_cap, (size_t)grid * 2 * a.place * 4));
+        a.part = dev->part_buf, a.arrived = dev->arrived;
+    }
+    const size_t lds = (size_t)NWV * heads * DP * 4;
+    const auto kern = k_paged_step<TX, TP, DP, NWV>;
+    FH_TRY(fh_kernel_lds(dev, (const void *)kern, lds));
+    kern<<<dim3(grid), dim3(64 * NWV), lds, dev->stream>>>(a);
+    FH_HIP(hipGetLastError());
+    return FH_OK;
+}
+template <typename TX, typename TP>
+static fh_status ps_dim(fh_device *dev, const PagedCall &call, int max_len) {
+    if (call.d <= 64) return ps_launch<TX, TP, 64, 8>(dev, call, max_len);
+    if (call.d <= 128) return ps_launch<TX, TP, 128, 8>(dev, call, max_len);
+    return ps_launch<TX, TP, 256, 4>(dev, call, max_len);
+}
+fh_status fh_paged_step(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len) {
+    if (dtype == FH_F16) return ps_dim<fh_half, fh_half>(dev, call, max_len);
+    if (dtype == FH_PAGED_BF16) return ps_dim<fh_bf, fh_bf>(dev, call, max_len);
+    if (kv_dtype == FH_F32) return ps_dim<float, float>(dev, call, max_len);
+    if (kv_dtype == FH_F16) return ps_dim<float, fh_half>(dev, call, max_len);
+    return ps_dim<float, fh_bf>(dev, call, max_len);
+}
