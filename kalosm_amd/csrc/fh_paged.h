@@ -59,6 +59,7 @@ struct PagedCall {
     int window, hq, hkv, d;
 };
 fh_status fh_paged_step(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len); // rows.max_new = 1
+fh_status fh_paged_prompt(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len);
 // The GPU of `dev` is the calling thread's current one while this lives.
 struct PagedGpu {
     int before = -1;

@@ -173,57 +173,6 @@ extern "C" fh_status fh_paged_rope_append(fh_device *dev, int32_t dtype, int32_t
 }
 
 // ---------------------------------------------------------------- attention
-// One wavefront a row and query head: a key a lane for the scores, a few values of the head a lane for the sums.
-template <typename TX, typename TP>
-__global__ __launch_bounds__(64) void k_paged_rows(const TX *__restrict__ q, int64_t q_st, int64_t q_sh, int hq, int hkv, int d, float scale, int window,
-                                                   PagedKv kv, PagedRows rows, TX *__restrict__ out) {
-    __shared__ float sq[256], sp[64];
-    __shared__ int64_t sa[64];
-    const int h = blockIdx.x, seq = blockIdx.z, lane = threadIdx.x;
-    const PagedSeq s = paged_seq(rows, kv.shift, seq);
-    if ((int)blockIdx.y >= s.rows) return;
-    const int row = s.row + blockIdx.y, p = s.first + (int)blockIdx.y, kh = h / (hq / hkv);
-    const int end = p + 1 < s.len ? p + 1 : s.len;
-    const int begin = window && p - window + 1 > 0 ? p - window + 1 : 0;
-    for (int e = lane; e < d; e += 64) sq[e] = (float)q[row * q_st + h * q_sh + e];
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int t = begin; t < end; t += 64) {
-        const int key = t + lane;
-        float x = -INFINITY;
-        int64_t at = -1;
-        if (key < end) {
-            const int page = rows.table[(int64_t)seq * rows.cols + (key >> kv.shift)];
-            if ((unsigned)page < (unsigned)kv.pages) {
-                at = (int64_t)page * kv.page + kh * kv.head + (int64_t)(key & ((1 << kv.shift) - 1)) * kv.slot;
-                const TP *kp = (const TP *)(kv.k + at);
-                x = 0.f;
-                for (int e = 0; e < d; e++) x = fmaf(sq[e], (float)kp[e], x);
-                x *= scale;
-            }
-        }
-        float mx = x;
-        for (int w = 32; w; w >>= 1) mx = fmaxf(mx, __shfl_xor(mx, w));
-        mx = fmaxf(mx, m);
-        const float ref = mx == -INFINITY ? 0.f : mx, alpha = expf(m - ref), pr = at < 0 ? 0.f : expf(x - ref);
-        m = mx;
-        float sum = pr;
-        for (int w = 32; w; w >>= 1) sum += __shfl_xor(sum, w);
-        l = l * alpha + sum;
-        sp[lane] = pr, sa[lane] = at;
-        __syncthreads();
-        for (int i = 0; i < 4; i++) o[i] *= alpha;
-        for (int j = 0; j < 64; j++)
-            if (sa[j] >= 0)
-                for (int i = 0; i < 4; i++)
-                    if (lane + 64 * i < d) o[i] = fmaf(sp[j], (float)((const TP *)(kv.v + sa[j]))[lane + 64 * i], o[i]);
-        __syncthreads();
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l; // a row that sees nothing: zeros
-    for (int i = 0; i < 4; i++)
-        if (lane + 64 * i < d) out[((int64_t)row * hq + h) * d + lane + 64 * i] = (TX)(o[i] * inv);
-}
-
 extern "C" fh_status fh_paged_attention(fh_device *dev, int32_t dtype, int32_t kv_dtype, const void *q_dev, int64_t q_st, int64_t q_sh, int32_t hq,
                                         int32_t hkv, int32_t d, float scale, int32_t window, const void *k_pages_dev, const void *v_pages_dev,
                                         int64_t page_stride, int64_t head_stride, int64_t slot_stride, int32_t pages, int32_t page_size,
@@ -243,15 +192,5 @@ extern "C" fh_status fh_paged_attention(fh_device *dev, int32_t dtype, int32_t k
     FH_TRY(gpu.enter(dev));
     const PagedCall call = {q_dev, out_dev, q_st, q_sh, kv, rows, scale, window, hq, hkv, d};
     if (rows.max_new == 1) return fh_paged_step(dev, dtype, kv_dtype, call, max_len);
-#define FH_PR(TX, TP)                                                                                                                              \
-    k_paged_rows<TX, TP><<<dim3((unsigned)hq, (unsigned)rows.max_new, (unsigned)seqs), dim3(64), 0, dev->stream>>>((const TX *)q_dev, q_st, q_sh, hq, hkv, d, scale,   \
-                                                                                                          window, kv, rows, (TX *)out_dev)
-    if (dtype == FH_F16) FH_PR(fh_half, fh_half);
-    else if (dtype == FH_PAGED_BF16) FH_PR(fh_bf, fh_bf);
-    else if (kv_dtype == FH_F32) FH_PR(float, float);
-    else if (kv_dtype == FH_F16) FH_PR(float, fh_half);
-    else FH_PR(float, fh_bf);
-#undef FH_PR
-    FH_HIP(hipGetLastError());
-    return FH_OK;
+    return fh_paged_prompt(dev, dtype, kv_dtype, call, max_len);
 }

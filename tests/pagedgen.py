@@ -103,22 +103,27 @@ class Pages:
                 o = w @ vs[:, h]
                 out[row, h * g:(h + 1) * g] = o
                 size = scale * (np.abs(x) @ np.abs(ks[:, h]).T).max(1, keepdims=True)
-                bound[row, h * g:(h + 1) * g] = attention_bound(o, w @ np.abs(vs[:, h]), size, len(j), self.d, self.act, self.kept)
+                bound[row, h * g:(h + 1) * g] = attention_bound(o, w @ np.abs(vs[:, h]), np.abs(vs[:, h]).sum(0), size, len(j), self.d, self.act, self.kept)
         return out, bound
 
 
-def attention_bound(o, mass, size, keys, d, act, kept):
-    """How far attention may be off: o the result, mass = sum w |v|, size = the largest scale * sum |q| |k| of a key.
+def attention_bound(o, mass, whole, size, keys, d, act, kept):
+    """How far attention may be off: o the result, mass = sum w |v|, whole = sum |v|, size = the largest scale * sum |q| |k| of a key.
 
     A score is a sum of d products held in f32, in any order, of operands whose terms carry 2^-23 of the value (f32 operands go to
     the matrix cores in parts), scaled once and taken to base 2: off by at most ds = (d + 6) 2^-23 size.  Normalised weights are
     then off by a factor within exp(+-2 ds), and the exponential itself by 2^-21.  Each weight is rounded to the type of the pages
     where it is multiplied in 16 bits (half a step; f32 rows: in several terms, 2^-22).  Sums over the keys are f32: each of
-    at most keys + 64 additions is off by 2^-24 of what has been summed, numerator and denominator alike.  The result is rounded once."""
+    at most keys + 64 additions is off by 2^-24 of what has been summed, numerator and denominator alike.  The result is rounded once.
+
+    Weights next to f16 values are f16 themselves, at 2^14 times their size relative to the largest (which is at most 1): where a term falls
+    below f16's normal range its half step is 2^-25, that is 2^-39 of a weight of 1, whatever the weight's own size - a result to which the heavy
+    positions contribute zeros can be off by that much of its small ones: 2^-39 sum |v| in all."""
     ds = (d + 6) * 2.0 ** -23 * size
     weight = HALF_STEP[kept] if act == kept and act != "f32" else 2.0 ** -22
     rel = np.expm1(2 * ds) + 2.0 ** -20 + weight + 2 * (keys + 64) * 2.0 ** -24
-    return 1.01 * (HALF_STEP[act] * (np.abs(o) + rel * mass) + rel * mass) + SMALLEST[act]
+    inner = rel * mass + (2.0 ** -39 * whole if kept == "f16" else 0.0)
+    return 1.01 * (HALF_STEP[act] * (np.abs(o) + inner) + inner) + SMALLEST[act]
 
 
 def near(got, want, bound, what):
