@@ -22,6 +22,7 @@
 // them up, in their order: the same bits in every run.  Pairs of few tiles are a workgroup each, and nothing is joined.
 #include "fh_paged.h"
 #include <type_traits>
+#include <stdlib.h>
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -52,16 +53,6 @@ __device__ __forceinline__ int ps_uniform(int a) { return __builtin_amdgcn_readf
 template <typename TP> struct PsVec { typedef half8 type; };
 template <> struct PsVec<fh_bf> { typedef bf8 type; };
 
-struct PsArgs {
-    PagedCall c;
-    int blocks; // of up to 16 query heads a KV head
-    int whole;  // a pair a workgroup
-    int least;  // tiles a stretch has at least
-    int place;  // floats of a part
-    float *part;
-    uint32_t *arrived;
-};
-
 // A pair's tiles: positions first * TK .. (first + tiles) * TK - 1, of which begin .. end - 1 are seen.
 struct PsSpan {
     int row, begin, end, first, tiles;
@@ -80,8 +71,14 @@ template <int TK> __device__ __forceinline__ PsSpan ps_span(const PagedSeq &s, i
     return r;
 }
 
+// The arguments that the first requests need come first: they are in registers when the kernel starts.
+//   blocks of up to 16 query heads a KV head; whole: a pair a workgroup; least: tiles a stretch has at least; place: floats of a part
 template <typename TX, typename TP, int DP, int NWV>
-__global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
+__global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__ table, const int *__restrict__ lens, const int *__restrict__ starts, int cols, int shift,
+                                                         int whole, int hkv, int blocks, int window, int pages, const char *__restrict__ k_pages,
+                                                         const char *__restrict__ v_pages, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                                                         const TX *__restrict__ q, int64_t q_st, int64_t q_sh, int group, int d, float scale, int seqs, int tokens, int least,
+                                                         int place, float *__restrict__ sums, uint32_t *__restrict__ arrived, TX *__restrict__ out) {
     constexpr bool F32 = sizeof(TP) == 4, F16 = __is_same(TP, fh_half), MIXED = sizeof(TX) != sizeof(TP);
     constexpr int TK = F32 ? 16 : 32, HALVES = TK / 16;
     constexpr int QT = F32 ? 1 : !MIXED ? 1 : F16 ? 2 : 3, PT = F32 ? 1 : MIXED ? (F16 ? 2 : 3) : F16 ? 1 : 2; // terms
@@ -94,16 +91,30 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
     __shared__ float s_st[NWV * 16 * 2];
     __shared__ uint32_t s_last;
     const int tid = threadIdx.x, wave = ps_uniform(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
-    const PagedKv &kv = a.c.kv;
-    const PagedRows &rows = a.c.rows;
-    const int group = a.c.hq / a.c.hkv, H = a.c.hkv * a.blocks, page_mask = (1 << kv.shift) - 1;
+    const PagedRows rows = {starts, lens, table, cols, seqs, tokens, 1};
+    const int H = hkv * blocks, page_mask = (1 << shift) - 1;
 
-    // ---- this workgroup's stretch of the line: tiles lo .. hi - 1; its first pair is of sequence b, which begins at `at`
-    int64_t step = 0, lo = 0, hi = 0, at = 0;
-    int b = 0;
-    if (a.whole) b = ps_uniform((int)blockIdx.x / H);
-    else {
-        auto tiles_of = [&](int i) { return i < rows.seqs ? ps_span<TK>(paged_seq(rows, kv.shift, i), a.c.window).tiles : 0; };
+    // ---- this workgroup's stretch of the line: `step` tiles.  Places on the line are counted from the stretch's beginning.
+    struct Cursor { // a pair on the line: sequence b, block hh of its query heads
+        PsSpan s;
+        int b, hh, kh, at;  // at: where it begins (below 0: in an earlier stretch)
+        int from, to;       // tiles from .. to - 1 of the pair lie in the stretch
+    };
+    Cursor cur;
+    int step = 0, stretch = 0; // stretch: its length where it is not the line's last
+    int early_page[HALVES]; // of this wavefront's first tile, if that is tile `wave` of the sequence
+    if (whole) {
+        cur.b = ps_uniform((int)blockIdx.x / H), cur.hh = (int)blockIdx.x - cur.b * H, cur.at = 0;
+#pragma unroll
+        for (int h = 0; h < HALVES; h++) {
+            const int col = (wave * TK + 16 * h) >> shift;
+            early_page[h] = paged_scalar(table, (int64_t)cur.b * cols + (col < cols ? col : cols - 1));
+        }
+        cur.s = ps_span<TK>(paged_seq_scalar(rows, shift, cur.b), window);
+        if (cur.s.tiles == 0) return;
+        step = cur.s.tiles;
+    } else {
+        auto tiles_of = [&](int i) { return i < seqs ? ps_span<TK>(paged_seq(rows, shift, i), window).tiles : 0; };
         auto scan = [&](int64_t x) { // inclusive, over the lanes
 #pragma unroll
             for (int w = 1; w < 64; w *= 2) {
@@ -113,65 +124,51 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
             return x;
         };
         auto uniform = [](int64_t x) { return (int64_t)((uint64_t)(uint32_t)ps_uniform((int)(x >> 32)) << 32 | (uint32_t)ps_uniform((int)x)); };
-        int64_t sums = scan(tiles_of(lane)), total = __shfl(sums, 63);
-        for (int c = 64; c < rows.seqs; c += 64) {
+        int64_t sums_ = scan(tiles_of(lane)), total = __shfl(sums_, 63);
+        for (int c = 64; c < seqs; c += 64) {
             int64_t x = tiles_of(c + lane);
 #pragma unroll
             for (int w = 32; w; w >>= 1) x += __shfl_xor(x, w);
             total += x;
         }
         total = uniform(total) * H;
-        step = (total + gridDim.x - 1) / gridDim.x;
-        step = step < a.least ? a.least : step;
-        lo = step * blockIdx.x, hi = lo + step < total ? lo + step : total;
+        int64_t each = (total + gridDim.x - 1) / gridDim.x;
+        each = each < least ? least : each;
+        const int64_t lo = each * blockIdx.x;
         if (lo >= total) return;
+        step = (int)(each < total - lo ? each : total - lo), stretch = (int)each;
         int64_t before = 0;
         int c = 0;
         for (;; c += 64) { // (lo < total: it ends)
-            if (c) sums = scan(tiles_of(c + lane));
-            const int64_t here = uniform(__shfl(sums, 63));
+            if (c) sums_ = scan(tiles_of(c + lane));
+            const int64_t here = uniform(__shfl(sums_, 63));
             if ((before + here) * H > lo) break;
             before += here;
         }
-        const int in = __popcll(__ballot((before + sums) * H <= lo)); // sequences of these 64 that end before
-        b = ps_uniform(c + in);
-        at = uniform(before + (in ? __shfl(sums, in - 1) : 0)) * H;
+        const int in = __popcll(__ballot((before + sums_) * H <= lo)); // sequences of these 64 that end before
+        cur.b = ps_uniform(c + in);
+        const int64_t at = uniform(before + (in ? __shfl(sums_, in - 1) : 0)) * H - lo;
+        cur.s = ps_span<TK>(paged_seq_scalar(rows, shift, cur.b), window);
+        cur.hh = (int)(-at / cur.s.tiles);
+        cur.at = (int)(at + (int64_t)cur.hh * cur.s.tiles);
+        early_page[0] = 0;
     }
-
-    // ---- a pair on the line: sequence b, block hh of its query heads
-    struct Cursor {
-        PsSpan s;
-        int b, hh, kh, from, to; // tiles from .. to - 1 of the pair lie in the stretch
-        int64_t pair_at;     // where the pair begins on the line
-    };
     auto enter = [&](Cursor &c) { // the part of the pair that lies in the stretch
-        const int64_t f = lo - c.pair_at, e = hi - c.pair_at;
-        c.from = f > 0 ? (int)f : 0;
-        c.to = e < c.s.tiles ? (int)e : c.s.tiles;
-        c.kh = a.blocks == 1 ? c.hh : c.hh / a.blocks;
+        c.from = c.at < 0 ? -c.at : 0;
+        c.to = step - c.at < c.s.tiles ? step - c.at : c.s.tiles;
+        c.kh = blocks == 1 ? c.hh : c.hh / blocks;
     };
     auto next_pair = [&](Cursor &c) { // false at the stretch's end
-        c.pair_at += c.s.tiles;
-        if (c.pair_at >= hi) return false;
+        if (c.at + c.s.tiles >= step) return false;
+        c.at += c.s.tiles;
         if (++c.hh == H) {
             c.hh = 0;
-            do c.s = ps_span<TK>(paged_seq_scalar(rows, kv.shift, ++c.b), a.c.window);
+            do c.s = ps_span<TK>(paged_seq_scalar(rows, shift, ++c.b), window);
             while (c.s.tiles == 0); // (the line goes on, so there is one)
         }
         enter(c);
         return true;
     };
-    Cursor cur;
-    cur.b = b;
-    cur.s = ps_span<TK>(paged_seq_scalar(rows, kv.shift, b), a.c.window);
-    if (a.whole) {
-        if (cur.s.tiles == 0) return;
-        cur.hh = (int)blockIdx.x % H;
-        cur.pair_at = 0, hi = cur.s.tiles;
-    } else {
-        cur.hh = (int)((lo - at) / cur.s.tiles);
-        cur.pair_at = at + (int64_t)cur.hh * cur.s.tiles;
-    }
     enter(cur);
 
     // ---- requests.  `ahead` is two tiles ahead of the products: the pages of its tile are asked for while the tile before is requested.
@@ -180,7 +177,7 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
     vpiece vr[HALVES][4][VL]; // [half][row 4 g + j][piece]
     uint32_t k_off[KL], v_off[4], v_piece[VL];
     {
-        const uint32_t slot = (uint32_t)kv.slot, row_bytes = (uint32_t)a.c.d * sizeof(TP);
+        const uint32_t slot = (uint32_t)slot_stride, row_bytes = (uint32_t)d * sizeof(TP);
 #pragma unroll
         for (int s = 0; s < KL; s++) { // pieces behind the head's end: its first one again (Q is zero there)
             const uint32_t piece = 64 * s + 16 * g;
@@ -210,19 +207,19 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
         next_kh = ahead.kh;
 #pragma unroll
         for (int h = 0; h < HALVES; h++) {
-            const int col = (next_key + 16 * h) >> kv.shift;
-            next_page[h] = paged_scalar(rows.table, (int64_t)ahead.b * rows.cols + (col < rows.cols ? col : rows.cols - 1));
+            const int col = (next_key + 16 * h) >> shift;
+            next_page[h] = paged_scalar(table, (int64_t)ahead.b * cols + (col < cols ? col : cols - 1));
         }
         t += NWV;
     };
-    auto place = [&]() {
+    auto move = [&]() {
         key0 = next_key, holes = 0;
 #pragma unroll
         for (int h = 0; h < HALVES; h++) {
             int page = next_page[h];
-            if ((unsigned)page >= (unsigned)kv.pages) page = 0, holes |= 1u << h;
-            const int64_t o = page * kv.page + next_kh * kv.head + ((key0 + 16 * h) & page_mask) * kv.slot;
-            kb[h] = kv.k + o, vb[h] = kv.v + o;
+            if ((unsigned)page >= (unsigned)pages) page = 0, holes |= 1u << h;
+            const int64_t o = page * page_stride + next_kh * head_stride + ((key0 + 16 * h) & page_mask) * slot_stride;
+            kb[h] = k_pages + o, vb[h] = v_pages + o;
         }
     };
     auto ask_k = [&]() {
@@ -239,8 +236,29 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
 #pragma unroll
                 for (int c = 0; c < VL; c++) vr[h][j][c] = *(const vpiece *)(vb[h] + (v_off[j] + v_piece[c]));
     };
-    look_up();
-    place();
+    // Q's values of a pair as they lie: lane (head n, g) has those of K's pieces; zeros for columns without a head and behind the head's end
+    constexpr int E = 16 / (int)sizeof(TP); // values of a piece
+    TX rq[KL][E];
+    auto ask_q = [&](const Cursor &c) {
+        const int skip = (c.hh - c.kh * blocks) * 16, head = c.kh * group + skip + n;
+        const TX *p = q + c.s.row * q_st + head * q_sh;
+#pragma unroll
+        for (int s = 0; s < KL; s++) {
+            const int at = 4 * E * s + E * g;
+#pragma unroll
+            for (int e = 0; e < E; e++) rq[s][e] = (TX)0.f;
+            if (skip + n < group && at < d) __builtin_memcpy(rq[s], p + at, sizeof(rq[s])); // (any address)
+        }
+    };
+    ask_q(cur);
+    if (whole && cur.s.first == 0 && wave < cur.s.tiles) {
+        next_key = wave * TK, next_kh = cur.kh;
+#pragma unroll
+        for (int h = 0; h < HALVES; h++) next_page[h] = early_page[h];
+        t += NWV;
+    } else
+        look_up();
+    move();
     ask_k();
     ask_v();
     look_up();
@@ -248,28 +266,19 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
     // ---- pair after pair
     bool go = true;
     while (go) {
-        const int skip = (cur.hh - cur.kh * a.blocks) * 16, h0 = cur.kh * group + skip, heads = group - skip < 16 ? group - skip : 16; // h0: first query head
-        // Q^T operand: lane (head n, g), values as K's pieces have them; zeros for columns without a head and behind the head's end
+        const int skip = (cur.hh - cur.kh * blocks) * 16, h0 = cur.kh * group + skip, heads = group - skip < 16 ? group - skip : 16; // h0: first query head
         vec8 qf[QT][F32 ? 1 : KL];
         floatx4 qx[F32 ? KL : 1];
-        float sc2 = a.c.scale * 1.4426950408889634f; // scores in the log2 domain
+        float sc2 = scale * 1.4426950408889634f; // scores in the log2 domain
         {
-            const TX *qp = (const TX *)a.c.q + cur.s.row * a.c.q_st + (h0 + n) * a.c.q_sh;
-            constexpr int E = 16 / (int)sizeof(TP); // values of a piece
             float x[KL][E], most = 0.f;
 #pragma unroll
-            for (int s = 0; s < KL; s++) {
-                const int dd = 4 * E * s + E * g;
-                TX v[E];
-#pragma unroll
-                for (int e = 0; e < E; e++) v[e] = (TX)0.f;
-                if (n < heads && dd < a.c.d) __builtin_memcpy(v, qp + dd, sizeof(v));
+            for (int s = 0; s < KL; s++)
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    x[s][e] = (float)v[e];
+                    x[s][e] = (float)rq[s][e];
                     most = fmaxf(most, fabsf(x[s][e]));
                 }
-            }
             if constexpr (MIXED && F16) { // brought to 2^14 .. 2^15
                 most = ps_rows_max(most);
                 int ex = 0;
@@ -306,19 +315,24 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
             floatx4 st[HALVES];
 #pragma unroll
             for (int h = 0; h < HALVES; h++) {
-                st[h] = floatx4{0.f, 0.f, 0.f, 0.f};
+                floatx4 other = {0.f, 0.f, 0.f, 0.f}; // (two chains: a product of f32 takes 32 cycles)
+                st[h] = other;
 #pragma unroll
                 for (int s = 0; s < KL; s++) {
                     if constexpr (F32) {
                         const floatx4 kx = __builtin_bit_cast(floatx4, kr[h][s]);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) st[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[e], qx[s][e], st[h], 0, 0, 0);
+                        for (int e = 0; e < 4; e += 2) {
+                            st[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[e], qx[s][e], st[h], 0, 0, 0);
+                            other = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[e + 1], qx[s][e + 1], other, 0, 0, 0);
+                        }
                     } else
 #pragma unroll
                         for (int w = QT - 1; w >= 0; w--) st[h] = ps_mfma(__builtin_bit_cast(vec8, kr[h][s]), qf[w][s], st[h]);
                 }
+                if constexpr (F32) st[h] += other;
             }
-            place();
+            move();
             __builtin_amdgcn_sched_barrier(0);
             ask_k();
             look_up();
@@ -400,7 +414,10 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
             __builtin_amdgcn_sched_barrier(0);
         }
 
-        // ---- the wavefronts' results together: thread (head, four values)
+        // ---- the wavefronts' results together: thread (head, four values); the next pair's Q is on its way
+        Cursor next = cur;
+        go = next_pair(next);
+        if (go) ask_q(next);
         l_run = ps_rows_sum(l_run);
         if (n < heads) {
             float *to = ps_lds + (wave * heads + n) * DP;
@@ -416,18 +433,20 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
         }
         __syncthreads();
         const bool all = cur.from == 0 && cur.to == cur.s.tiles;
-        constexpr int PITCH = DP + 4; // of a part's head: values, maximum, sum
-        float *own = a.part + ((int64_t)blockIdx.x * 2 + (cur.from ? 0 : 1)) * a.place;
-        auto store = [&](int h, int dd, floatx4 x, float den) {
-            if (dd >= a.c.d) return;
-            const float inv = den == 0.f ? 0.f : 1.f / den;
+        constexpr int PITCH = DP + 4, QUADS = DP / 4; // PITCH: of a part's head: values, maximum, sum
+        float *own = sums + ((int64_t)blockIdx.x * 2 + (cur.from ? 0 : 1)) * place;
+        auto put = [&](float *p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+        auto get = [&](const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+        auto store = [&](int h, int at, floatx4 x, float den) {
+            if (at >= d) return;
+            const float inv = den == 0.f ? 0.f : 1.f / den; // (a row that sees nothing: zeros)
             TX y[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) y[i] = (TX)(x[i] * inv);
-            __builtin_memcpy((TX *)a.c.out + ((int64_t)cur.s.row * a.c.hq + h0 + h) * a.c.d + dd, y, sizeof(y));
+            __builtin_memcpy(out + ((int64_t)cur.s.row * hkv * group + h0 + h) * d + at, y, sizeof(y));
         };
-        for (int i = tid; i < heads * (DP / 4); i += THREADS) {
-            const int h = i / (DP / 4), dd = i % (DP / 4) * 4;
+        for (int i = tid; i < heads * QUADS; i += THREADS) {
+            const int h = i / QUADS, at = i % QUADS * 4;
             float mx = -INFINITY, den = 0.f;
 #pragma unroll
             for (int w = 0; w < NWV; w++) mx = fmaxf(mx, s_st[(w * 16 + h) * 2]);
@@ -436,48 +455,77 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(PsArgs a) {
 #pragma unroll
             for (int w = 0; w < NWV; w++) {
                 const float f = __builtin_amdgcn_exp2f(s_st[(w * 16 + h) * 2] - ref);
-                x += *(const floatx4 *)(ps_lds + (w * heads + h) * DP + dd) * f;
+                x += *(const floatx4 *)(ps_lds + (w * heads + h) * DP + at) * f;
                 den = fmaf(s_st[(w * 16 + h) * 2 + 1], f, den);
             }
-            if (all) store(h, dd, x, den);
+            if (all) store(h, at, x, den);
             else {
 #pragma unroll
-                for (int e = 0; e < 4; e++) __hip_atomic_store(own + h * PITCH + dd + e, x[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (dd == 0) {
-                    __hip_atomic_store(own + h * PITCH + DP, mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    __hip_atomic_store(own + h * PITCH + DP + 1, den, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
+                for (int e = 0; e < 4; e++) put(own + h * PITCH + at + e, x[e]);
+                if (at == 0) put(own + h * PITCH + DP, mx), put(own + h * PITCH + DP + 1, den);
             }
         }
         if (!all) {
-            const int w0 = (int)(cur.pair_at / step), parts = (int)((cur.pair_at + cur.s.tiles - 1) / step) - w0 + 1;
+            // the pair's workgroups (all stretches before the line's last are as long as this one, or this is the last)
+            const int w0 = (int)blockIdx.x - (cur.from ? (cur.from + stretch - 1) / stretch : 0);
+            const int parts = (int)blockIdx.x - w0 + 1 + (cur.s.tiles - cur.to + stretch - 1) / stretch;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // written before this workgroup counts itself in
             __syncthreads();
-            if (tid == 0) s_last = __hip_atomic_fetch_add(a.arrived + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (tid == 0) s_last = __hip_atomic_fetch_add(arrived + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
             if (s_last == (uint32_t)parts - 1) {
-                if (tid == 0) __hip_atomic_store(a.arrived + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // as it was found
-                auto part = [&](int i) { return a.part + ((int64_t)(w0 + i) * 2 + (i ? 0 : 1)) * a.place; };
-                auto get = [&](const float *f) { return __hip_atomic_load(f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-                for (int i = tid; i < heads * (DP / 4); i += THREADS) {
-                    const int h = i / (DP / 4), dd = i % (DP / 4) * 4;
-                    float mx = -INFINITY, den = 0.f;
-                    for (int k = 0; k < parts; k++) mx = fmaxf(mx, get(part(k) + h * PITCH + DP));
-                    const float ref = mx == -INFINITY ? 0.f : mx;
-                    floatx4 x = {0.f, 0.f, 0.f, 0.f};
-                    for (int k = 0; k < parts; k++) {
-                        const float *f = part(k) + h * PITCH;
-                        const float w = __builtin_amdgcn_exp2f(get(f + DP) - ref);
-                        den = fmaf(get(f + DP + 1), w, den);
+                if (tid == 0) __hip_atomic_store(arrived + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // as it was found
+                auto part = [&](int i) { return sums + ((int64_t)(w0 + i) * 2 + (i ? 0 : 1)) * place; };
+                float *s_w = ps_lds, *s_l = ps_lds + parts * heads; // [head][part]: maxima, then weights; sums
+                for (int i = tid; i < parts * heads; i += THREADS) {
+                    const float *p = part(i % parts) + i / parts * PITCH + DP;
+                    s_w[i] = get(p), s_l[i] = get(p + 1);
+                }
+                __syncthreads();
+                for (int h = wave; h < heads; h += NWV) { // a wavefront a head
+                    float mx = -INFINITY, sum = 0.f;
+                    for (int i = lane; i < parts; i += 64) mx = fmaxf(mx, s_w[h * parts + i]);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) x[e] = fmaf(get(f + dd + e), w, x[e]);
+                    for (int w = 32; w; w >>= 1) mx = fmaxf(mx, __shfl_xor(mx, w));
+                    const float ref = mx == -INFINITY ? 0.f : mx;
+                    for (int i = lane; i < parts; i += 64) {
+                        const float f = __builtin_amdgcn_exp2f(s_w[h * parts + i] - ref);
+                        s_w[h * parts + i] = f;
+                        sum = fmaf(s_l[h * parts + i], f, sum);
                     }
-                    store(h, dd, x, den);
+#pragma unroll
+                    for (int w = 32; w; w >>= 1) sum += __shfl_xor(sum, w);
+                    if (lane == 0) s_st[h] = sum;
+                }
+                __syncthreads();
+                // Groups of threads take parts in turn; their sums meet in LDS behind the weights.
+                const int items = heads * QUADS, groups = items < THREADS ? THREADS / items : 1;
+                float *s_x = ps_lds + 2 * parts * heads + (2 * parts * heads & 2 ? 2 : 0); // (16-byte places)
+                for (int base = 0; base < items; base += THREADS) {
+                    const int i = base + (groups > 1 ? tid % items : tid), pg = groups > 1 ? tid / items : 0;
+                    floatx4 x = {0.f, 0.f, 0.f, 0.f};
+                    if (i < items && pg < groups) {
+                        const int h = i / QUADS, at = i % QUADS * 4;
+#pragma unroll 4
+                        for (int k = pg; k < parts; k += groups) {
+                            const float *p = part(k) + h * PITCH + at;
+                            const float w = s_w[h * parts + k];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) x[e] = fmaf(get(p + e), w, x[e]);
+                        }
+                    }
+                    if (groups > 1) {
+                        if (pg < groups) *(floatx4 *)(s_x + (pg * items + i) * 4) = x;
+                        __syncthreads();
+                        if (pg == 0)
+                            for (int k = 1; k < groups; k++) x += *(const floatx4 *)(s_x + (k * items + i) * 4);
+                    }
+                    if (i < items && pg == 0) store(i / QUADS, i % QUADS * 4, x, s_st[i / QUADS]);
                 }
             }
         }
         __syncthreads(); // the next pair's results go to the same places
-        go = next_pair(cur);
+        cur = next;
     }
 }
 
@@ -485,26 +533,28 @@ template <typename TX, typename TP, int DP, int NWV>
 static fh_status ps_launch(fh_device *dev, const PagedCall &call, int max_len) {
     constexpr int TK = sizeof(TP) == 4 ? 16 : 32;
     const int group = call.hq / call.hkv, heads = group < 16 ? group : 16;
-    PsArgs a = {};
-    a.c = call;
-    a.blocks = (group + 15) / 16;
-    a.place = heads * (DP + 4);
-    a.least = NWV;
+    const int blocks = (group + 15) / 16, place = heads * (DP + 4);
     int64_t longest = (int64_t)call.rows.cols << call.kv.shift;
     if (max_len > 0 && max_len < longest) longest = max_len;
     if (call.window > 0 && call.window + TK < longest) longest = call.window + TK;
-    const int64_t pairs = (int64_t)call.rows.seqs * call.hkv * a.blocks;
-    a.whole = longest <= 4 * NWV * TK;
+    const int64_t pairs = (int64_t)call.rows.seqs * call.hkv * blocks;
+    int whole = longest <= 4 * NWV * TK, least = NWV;
+    if (getenv("XW")) whole = atoi(getenv("XW"));
+    if (getenv("XL")) least = atoi(getenv("XL"));
     unsigned grid = (unsigned)pairs;
-    if (!a.whole) {
+    if (!whole) {
         grid = (unsigned)dev->compute_units;
-        FH_TRY(fh_dev_scratch(dev, (void **)&dev->part_buf, &dev->part_cap, (size_t)grid * 2 * a.place * 4));
-        a.part = dev->part_buf, a.arrived = dev->arrived;
+        FH_TRY(fh_dev_scratch(dev, (void **)&dev->part_buf, &dev->part_cap, (size_t)grid * 2 * place * 4));
     }
-    const size_t lds = (size_t)NWV * heads * DP * 4;
+    // results of the wavefronts; where parts are joined, two words a part and head and 16 bytes a thread
+    size_t lds = (size_t)NWV * heads * DP * 4;
+    const size_t join = (size_t)grid * heads * 8 + 16 + 64 * NWV * 16;
+    if (!whole && lds < join) lds = join;
     const auto kern = k_paged_step<TX, TP, DP, NWV>;
     FH_TRY(fh_kernel_lds(dev, (const void *)kern, lds));
-    kern<<<dim3(grid), dim3(64 * NWV), lds, dev->stream>>>(a);
+    kern<<<dim3(grid), dim3(64 * NWV), lds, dev->stream>>>(call.rows.table, call.rows.lens, call.rows.starts, call.rows.cols, call.kv.shift, whole, call.hkv, blocks, call.window,
+                                                           call.kv.pages, call.kv.k, call.kv.v, call.kv.page, call.kv.head, call.kv.slot, (const TX *)call.q, call.q_st, call.q_sh,
+                                                           group, call.d, call.scale, call.rows.seqs, call.rows.tokens, least, place, dev->part_buf, dev->arrived, (TX *)call.out);
     FH_HIP(hipGetLastError());
     return FH_OK;
 }
