@@ -5,7 +5,7 @@
 typedef _Float16 fh_half;
 typedef __bf16 fh_bf;
 
-enum { FH_PAGED_BF16 = FH_DECODER_BF16, FH_PAGED_MAX = 1 << 30 /* positions of a sequence */ };
+enum { FH_PAGED_BF16 = FH_DECODER_BF16, FH_PAGED_MAX = 1 << 29 /* positions of a sequence */ };
 
 struct PagedKv {
     const char *k, *v;

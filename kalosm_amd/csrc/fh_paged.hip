@@ -31,8 +31,8 @@ fh_status fh_paged_arguments(int dtype, int kv_dtype, int hq, int hkv, int d, co
     if (d % 8 || d > 256) FH_FAIL(FH_ERR_UNSUPPORTED, "head_dim %d: paged attention takes multiples of 8 up to 256", d);
     if (page_size < 16 || page_size > 4096 || (page_size & (page_size - 1)))
         FH_FAIL(FH_ERR_UNSUPPORTED, "pages of %d positions: powers of two from 16 to 4096 are supported", page_size);
-    FH_REQUIRE(hq <= 65535 && seqs <= 65535 && pages <= FH_PAGED_MAX, "at most 65535 heads and sequences and 2^30 pages");
-    FH_REQUIRE((int64_t)cols * page_size <= FH_PAGED_MAX, "a table row of %d pages of %d positions reaches past 2^30", cols, page_size);
+    FH_REQUIRE(hq <= 65535 && seqs <= 65535 && pages <= FH_PAGED_MAX, "at most 65535 heads and sequences and 2^29 pages");
+    FH_REQUIRE((int64_t)cols * page_size <= FH_PAGED_MAX, "a table row of %d pages of %d positions reaches past 2^29", cols, page_size);
     FH_REQUIRE(starts || tokens == seqs, "%d rows of %d sequences need their starts", tokens, seqs);
     const int size = kv_dtype == FH_F32 ? 4 : 2;
     const int64_t lim = INT64_MAX / 8 / pages / size;

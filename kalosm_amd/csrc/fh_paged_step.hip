@@ -50,6 +50,18 @@ __device__ __forceinline__ floatx4 ps_mfma(half8 a, half8 b, floatx4 c) { return
 __device__ __forceinline__ floatx4 ps_mfma(bf8 a, bf8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ int ps_uniform(int a) { return __builtin_amdgcn_readfirstlane(a); }
 
+__device__ __forceinline__ uint32_t ps_scan(uint32_t x) { // inclusive prefix sums over the lanes
+#define PS_ADD(CTRL, ROWS) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false)
+    PS_ADD(0x111, 0xf); // within 16 lanes: from 1, 2, 4, 8 before
+    PS_ADD(0x112, 0xf);
+    PS_ADD(0x114, 0xf);
+    PS_ADD(0x118, 0xf);
+    PS_ADD(0x142, 0xa); // rows 1 and 3: the last lane of the row before
+    PS_ADD(0x143, 0xc); // rows 2 and 3: lane 31
+#undef PS_ADD
+    return x;
+}
+
 template <typename TP> struct PsVec { typedef half8 type; };
 template <> struct PsVec<fh_bf> { typedef bf8 type; };
 
@@ -114,24 +126,17 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
         if (cur.s.tiles == 0) return;
         step = cur.s.tiles;
     } else {
-        auto tiles_of = [&](int i) { return i < seqs ? ps_span<TK>(paged_seq(rows, shift, i), window).tiles : 0; };
-        auto scan = [&](int64_t x) { // inclusive, over the lanes
-#pragma unroll
-            for (int w = 1; w < 64; w *= 2) {
-                const int64_t y = __shfl_up(x, w);
-                if (lane >= w) x += y;
-            }
-            return x;
+        // Prefix sums over 64 sequences at a time; a sequence has fewer than 2^26 tiles.
+        PsSpan mine = {};
+        auto tiles_of = [&](int i) {
+            if (i >= seqs) return 0u;
+            mine = ps_span<TK>(paged_seq(rows, shift, i), window);
+            return (uint32_t)mine.tiles;
         };
-        auto uniform = [](int64_t x) { return (int64_t)((uint64_t)(uint32_t)ps_uniform((int)(x >> 32)) << 32 | (uint32_t)ps_uniform((int)x)); };
-        int64_t sums_ = scan(tiles_of(lane)), total = __shfl(sums_, 63);
-        for (int c = 64; c < seqs; c += 64) {
-            int64_t x = tiles_of(c + lane);
-#pragma unroll
-            for (int w = 32; w; w >>= 1) x += __shfl_xor(x, w);
-            total += x;
-        }
-        total = uniform(total) * H;
+        uint32_t upto = ps_scan(tiles_of(lane)), here = ps_uniform(__builtin_amdgcn_readlane(upto, 63));
+        int64_t total = here;
+        for (int c = 64; c < seqs; c += 64) total += (uint32_t)__builtin_amdgcn_readlane(ps_scan(tiles_of(c + lane)), 63);
+        total *= H;
         int64_t each = (total + gridDim.x - 1) / gridDim.x;
         each = each < least ? least : each;
         const int64_t lo = each * blockIdx.x;
@@ -139,16 +144,17 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
         step = (int)(each < total - lo ? each : total - lo), stretch = (int)each;
         int64_t before = 0;
         int c = 0;
-        for (;; c += 64) { // (lo < total: it ends)
-            if (c) sums_ = scan(tiles_of(c + lane));
-            const int64_t here = uniform(__shfl(sums_, 63));
-            if ((before + here) * H > lo) break;
-            before += here;
-        }
-        const int in = __popcll(__ballot((before + sums_) * H <= lo)); // sequences of these 64 that end before
+        if (seqs > 64) // (lo < total: it ends)
+            for (;; c += 64) {
+                upto = ps_scan(tiles_of(c + lane)), here = __builtin_amdgcn_readlane(upto, 63);
+                if ((before + here) * H > lo) break;
+                before += here;
+            }
+        const int in = __popcll(__ballot((before + upto) * H <= lo)); // sequences of these 64 that end before
         cur.b = ps_uniform(c + in);
-        const int64_t at = uniform(before + (in ? __shfl(sums_, in - 1) : 0)) * H - lo;
-        cur.s = ps_span<TK>(paged_seq_scalar(rows, shift, cur.b), window);
+        cur.s.row = __builtin_amdgcn_readlane(mine.row, in), cur.s.begin = __builtin_amdgcn_readlane(mine.begin, in), cur.s.end = __builtin_amdgcn_readlane(mine.end, in);
+        cur.s.first = __builtin_amdgcn_readlane(mine.first, in), cur.s.tiles = __builtin_amdgcn_readlane(mine.tiles, in);
+        const int64_t at = (before + (in ? (uint32_t)__builtin_amdgcn_readlane(upto, in - 1) : 0u)) * H - lo;
         cur.hh = (int)(-at / cur.s.tiles);
         cur.at = (int)(at + (int64_t)cur.hh * cur.s.tiles);
         early_page[0] = 0;
@@ -477,6 +483,20 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
                 if (tid == 0) __hip_atomic_store(arrived + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // as it was found
                 auto part = [&](int i) { return sums + ((int64_t)(w0 + i) * 2 + (i ? 0 : 1)) * place; };
                 float *s_w = ps_lds, *s_l = ps_lds + parts * heads; // [head][part]: maxima, then weights; sums
+                // Groups of threads take parts in turn, the first EARLY of each along with the statistics.
+                const int items = heads * QUADS, groups = items < THREADS ? THREADS / items : 1, pg = groups > 1 ? tid / items : 0;
+                constexpr int EARLY = MIXED && !F16 ? 4 : 8;
+                floatx4 first[EARLY];
+                auto ask = [&](int i, int k) {
+                    const float *p = part(k) + i / QUADS * PITCH + i % QUADS * 4;
+                    return floatx4{get(p), get(p + 1), get(p + 2), get(p + 3)};
+                };
+                {
+                    const int i = groups > 1 ? tid % items : tid;
+#pragma unroll
+                    for (int k = 0; k < EARLY; k++)
+                        if (pg + k * groups < parts && i < items && pg < groups) first[k] = ask(i, pg + k * groups);
+                }
                 for (int i = tid; i < parts * heads; i += THREADS) {
                     const float *p = part(i % parts) + i / parts * PITCH + DP;
                     s_w[i] = get(p), s_l[i] = get(p + 1);
@@ -498,21 +518,17 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
                     if (lane == 0) s_st[h] = sum;
                 }
                 __syncthreads();
-                // Groups of threads take parts in turn; their sums meet in LDS behind the weights.
-                const int items = heads * QUADS, groups = items < THREADS ? THREADS / items : 1;
                 float *s_x = ps_lds + 2 * parts * heads + (2 * parts * heads & 2 ? 2 : 0); // (16-byte places)
                 for (int base = 0; base < items; base += THREADS) {
-                    const int i = base + (groups > 1 ? tid % items : tid), pg = groups > 1 ? tid / items : 0;
+                    const int i = base + (groups > 1 ? tid % items : tid);
                     floatx4 x = {0.f, 0.f, 0.f, 0.f};
                     if (i < items && pg < groups) {
-                        const int h = i / QUADS, at = i % QUADS * 4;
-#pragma unroll 4
-                        for (int k = pg; k < parts; k += groups) {
-                            const float *p = part(k) + h * PITCH + at;
-                            const float w = s_w[h * parts + k];
+                        const float *w = s_w + i / QUADS * parts;
 #pragma unroll
-                            for (int e = 0; e < 4; e++) x[e] = fmaf(get(p + e), w, x[e]);
-                        }
+                        for (int k = 0; k < EARLY; k++)
+                            if (pg + k * groups < parts) x += (base ? ask(i, pg + k * groups) : first[k]) * w[pg + k * groups];
+#pragma unroll 4
+                        for (int k = pg + EARLY * groups; k < parts; k += groups) x += ask(i, k) * w[k];
                     }
                     if (groups > 1) {
                         if (pg < groups) *(floatx4 *)(s_x + (pg * items + i) * 4) = x;
