@@ -14,6 +14,7 @@
 // what it sees (pp_again): one at a time by a wavefront, slow, and never entered by finite caches.
 #include "fh_attention_tiles.h"
 #include "fh_paged.h"
+#include <stdlib.h>
 #include <type_traits>
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
@@ -147,12 +148,13 @@ __device__ __forceinline__ void pp_check(const PpArgs &a, int part, int seq, con
 // ---------------------------------------------------------------- rows and pages of one 16-bit type, head_dim 64 or 128
 // k_attn_ahead's loop (fh_attention_prefill.hip): the scores of the next tile beside the softmax of this one, K a tile ahead of V, both straight
 // into LDS with their 16-byte pieces swapped on the memory side.
-template <typename T, int D, int KS, int QW>
-__global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW == 4 ? 2 : 1, 2))) void k_paged_tiles(PpArgs a) {
+// NB buffers: step `it` asks for K of step it + NB and V of step it + NB - 1.
+template <typename T, int D, int KS, int QW, int NB>
+__global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW >= 4 ? 2 : 1, 2))) void k_paged_tiles(PpArgs a) {
     constexpr int BN = 64, DT = D / 32, KSTEPS = D / 16, CH = D / 8, TILE = BN * D, NW = QW * KS, NP = TILE * KS * 2 / 1024 / NW; // NP: 1 KB pieces of K a wavefront
     constexpr bool F16 = __is_same(T, fh_half);
     typedef typename PpVec<T>::type vec8;
-    extern __shared__ __attribute__((aligned(16))) fh_half pp_lds[]; // [2 buffers][KS tiles of K, KS of V]
+    extern __shared__ __attribute__((aligned(16))) fh_half pp_lds[]; // [NB buffers][KS tiles of K, KS of V]
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, li = lane & 31, g = lane >> 5;
     const int kset = KS == 2 ? wave / QW : 0;
     const PagedKv &kv = a.c.kv;
@@ -190,7 +192,7 @@ __global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW
         }
     };
     auto fetch = [&](const char *base, int c, int it, int plane, const int64_t (&at)[NP]) __attribute__((always_inline)) { // step `it` of K (plane 0) or V (1) into its buffer
-        fh_half *to = pp_lds + ((it & 1) * 2 + plane) * KS * TILE + wave * 512;
+        fh_half *to = pp_lds + (it % NB * 2 + plane) * KS * TILE + wave * 512;
         if (span.base + (it + 1) * KS * BN <= s.len) {
 #pragma unroll
             for (int i = 0; i < NP; i++) fh_buffer_to_lds(base + at[i], 0x7FFFFFFF, to + NW * i * 512, (row & 15) * slot + c, 0);
@@ -202,19 +204,37 @@ __global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW
             }
         }
     };
-    auto landed = [&]() { // this wavefront's pieces, and everybody's behind the barrier
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // This wavefront's pieces but the LATER last requests' are there, and everybody's behind the barrier; where no more are asked for, all of them.
+    auto landed = [&](auto later, bool asking) {
+        if (decltype(later)::value > 0 && asking) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(later)::value) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
+    constexpr std::integral_constant<int, (2 * NB - 2) * NP> but_first = {};
+    constexpr std::integral_constant<int, (2 * NB - 4) * NP> but_two = {}; // K of the first two steps and V of the first, or a step's requests of NB - 2 steps
+    static_assert((2 * NB - 2) * NP < 64, "a counter of six bits");
+    // Whether any entry of the table that this part reads is no page; only then are they looked at again where scores are masked.
+    bool holed = false;
+    if (steps > 0) {
+        const int c0 = span.base >> kv.shift, p1 = span.base + steps * KS * BN - 1, c1 = (p1 < s.len - 1 ? p1 : s.len - 1) >> kv.shift;
+        for (int c = c0 + lane; c <= c1; c += 64) holed |= (unsigned)rows.table[(int64_t)seq * rows.cols + c] >= (unsigned)kv.pages;
+        holed = __any(holed);
+    }
     int page[NP];
     int64_t now[NP], then[NP]; // of the step whose V is requested next, and of the one whose K is
-    if (steps > 0) {
-        look(0, page);
-        place(0, page, now);
-        fetch(kv.k, kc, 0, 0, now), fetch(kv.v, vc, 0, 1, now);
-        if (steps > 1) look(1, page);
-    }
+    if (steps > 0) look(0, page);
+#pragma unroll
+    for (int j = 0; j < NB; j++)
+        if (j < steps) {
+            place(j, page, then);
+            if (j + 1 < steps) look(j + 1, page);
+            fetch(kv.k, kc, j, 0, then);
+            if (j > 0) fetch(kv.v, vc, j - 1, 1, now);
+#pragma unroll
+            for (int i = 0; i < NP; i++) now[i] = then[i];
+        }
+    if (steps < NB && steps > 0) fetch(kv.v, vc, steps - 1, 1, now);
     vec8 qf[KSTEPS];
     {
         const T *qp = (const T *)a.c.q + (s.row + x.token) * a.c.q_st + (kh * group + x.head) * a.c.q_sh + 8 * g;
@@ -233,7 +253,7 @@ __global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) acc[dt] = zero;
     auto scores = [&](int it, floatx16 (&to)[2]) __attribute__((always_inline)) { // S^T of step `it`
-        uint32_t at = k_at + (uint32_t)(it & 1) * (4 * KS * TILE); // (swapped pieces are an exclusive or on the address, one instruction where it is used)
+        uint32_t at = k_at + (uint32_t)(it % NB) * (4 * KS * TILE); // (swapped pieces are an exclusive or on the address, one instruction where it is used)
         asm volatile("" : "+v"(at));
         constexpr int NI = 2 * KSTEPS, AHEAD = 4;
         vec8 ka[AHEAD];
@@ -250,6 +270,7 @@ __global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW
     auto mask = [&](int it, floatx16 (&to)[2]) __attribute__((always_inline)) {
         const int t0 = span.base + (it * KS + kset) * BN;
         uint32_t holes = 0; // its 16s without a page
+        if (holed)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int p = t0 + 16 * i;
@@ -265,14 +286,14 @@ __global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW
                     to[kt][r] = seen ? to[kt][r] : -INFINITY;
                 }
     };
-    auto requests = [&](int it) __attribute__((always_inline)) { // K of the step after the next, V of the next
-        if (it + 2 < steps) {
-            place(it + 2, page, then);
-            fetch(kv.k, kc, it + 2, 0, then);
-            if (it + 3 < steps) look(it + 3, page);
+    auto requests = [&](int it) __attribute__((always_inline)) {
+        if (it + NB < steps) {
+            place(it + NB, page, then);
+            fetch(kv.k, kc, it + NB, 0, then);
+            if (it + NB + 1 < steps) look(it + NB + 1, page);
         }
-        if (it + 1 < steps) {
-            fetch(kv.v, vc, it + 1, 1, now);
+        if (it + NB - 1 < steps) {
+            fetch(kv.v, vc, it + NB - 1, 1, now);
 #pragma unroll
             for (int i = 0; i < NP; i++) now[i] = then[i];
         }
@@ -310,6 +331,10 @@ __global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW
                     pb[kt][s2][e] = (T)p;
                 }
         l_run += ps;
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) // (here, beside the scores, and not behind the branch that follows)
+#pragma unroll
+            for (int s2 = 0; s2 < 2; s2++) asm volatile("" : "+v"(pb[kt][s2]));
         if (!last) {
             __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
@@ -323,7 +348,7 @@ __global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW
         __builtin_amdgcn_sched_barrier(0);
         if (!last) mask(it + 1, next);
         __builtin_amdgcn_sched_barrier(0);
-        uint32_t at = v_at + (uint32_t)(it & 1) * (4 * KS * TILE);
+        uint32_t at = v_at + (uint32_t)(it % NB) * (4 * KS * TILE);
         asm volatile("" : "+v"(at));
         constexpr int NJ = 4 * DT, AHEAD = 8;
         half8 va[AHEAD];
@@ -343,21 +368,14 @@ __global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
-        landed();
+        landed(but_two, it + NB < steps);
     };
     if (steps > 0) {
-        landed();
-        if (steps > 1) {
-            place(1, page, then);
-            fetch(kv.k, kc, 1, 0, then);
-            if (steps > 2) look(2, page);
-#pragma unroll
-            for (int i = 0; i < NP; i++) now[i] = then[i];
-        }
+        landed(but_first, steps >= NB);
         if (alive) {
             scores(0, sa);
             mask(0, sa);
-            landed(); // (K of step 1; the place of step 0's is free)
+            landed(but_two, steps >= NB);
             int t = 0;
             for (; t + 2 < steps; t += 2) {
                 step(t, sa, sb, false);
@@ -369,10 +387,10 @@ __global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW
             } else
                 step(t, sa, sb, true);
         } else {
-            landed();
+            landed(but_two, steps >= NB);
             for (int t = 0; t < steps; t++) {
                 requests(t);
-                landed();
+                landed(but_two, t + NB < steps);
             }
         }
     }
@@ -615,10 +633,11 @@ __global__ __launch_bounds__(256) void k_paged_join(PpArgs a) {
 }
 
 // ---------------------------------------------------------------- which form
-// Parts: a power of two that brings the workgroups to two a compute unit, each with at least `least` positions; scratch memory that cannot be had: one.
+// Parts: as many as compute units have a workgroup each, with at least `least` positions; where scratch memory cannot be had, one.
 static int pp_parts(fh_device *dev, const PagedCall &call, int64_t wgs, int64_t longest, int least, PpArgs *a) {
-    int parts = 1;
-    while (wgs * parts < dev->compute_units && longest / (2 * parts) >= least) parts *= 2;
+    int parts = (int)(dev->compute_units / wgs);
+    parts = (int)(longest / least < parts ? longest / least : parts);
+    parts = parts < 1 ? 1 : parts;
     a->parts = parts;
     if (parts == 1) return 1;
     const size_t n = (size_t)parts * call.rows.tokens * call.hq;
@@ -634,10 +653,10 @@ template <typename TX> static fh_status pp_join(fh_device *dev, const PpArgs &a)
     return FH_OK;
 }
 
-template <typename T, int D, int KS, int QW>
+template <typename T, int D, int KS, int QW, int NB>
 static fh_status pp_tiles(fh_device *dev, PpArgs a) {
-    constexpr int LDS = 2 * 2 * KS * 64 * D * 2, MERGE = KS == 2 ? (2 + D / 2) * 64 * QW * 4 : 0, BYTES = LDS > MERGE ? LDS : MERGE;
-    const auto kern = k_paged_tiles<T, D, KS, QW>;
+    constexpr int LDS = NB * 2 * KS * 64 * D * 2, MERGE = KS == 2 ? (2 + D / 2) * 64 * QW * 4 : 0, BYTES = LDS > MERGE ? LDS : MERGE;
+    const auto kern = k_paged_tiles<T, D, KS, QW, NB>;
     FH_TRY(fh_kernel_lds(dev, (const void *)kern, BYTES));
     const unsigned blocks = (unsigned)(((int64_t)a.c.rows.max_new * (a.c.hq / a.c.hkv) + 32 * QW - 1) / (32 * QW));
     kern<<<dim3((unsigned)a.c.hkv, blocks, (unsigned)(a.c.rows.seqs * a.parts)), dim3(64 * QW * KS), BYTES, dev->stream>>>(a);
@@ -663,11 +682,14 @@ template <typename TX, typename TP> static fh_status pp_dim(fh_device *dev, cons
 template <typename T> static fh_status pp_same(fh_device *dev, PpArgs a, int64_t longest) {
     if (a.c.d != 64 && a.c.d != 128) return pp_dim<T, T>(dev, a, longest);
     const int64_t rows = (int64_t)a.c.rows.max_new * (a.c.hq / a.c.hkv), pairs = (int64_t)a.c.hkv * a.c.rows.seqs;
-    const int64_t wgs = pairs * ((rows + 127) / 128), wgs64 = pairs * ((rows + 63) / 64);
-    const bool halves = wgs <= 2 * dev->compute_units && longest > 128, rows64 = halves && 4 * wgs64 <= 5 * dev->compute_units;
-    pp_parts(dev, a.c, rows64 ? wgs64 : wgs, longest, 512, &a);
-    if (a.c.d == 128) return rows64 ? pp_tiles<T, 128, 2, 2>(dev, a) : halves ? pp_tiles<T, 128, 2, 4>(dev, a) : pp_tiles<T, 128, 1, 4>(dev, a);
-    return rows64 ? pp_tiles<T, 64, 2, 2>(dev, a) : halves ? pp_tiles<T, 64, 2, 4>(dev, a) : pp_tiles<T, 64, 1, 4>(dev, a);
+    const int64_t wgs = pairs * ((rows + 127) / 128), wgs64 = pairs * ((rows + 63) / 64), wgs256 = pairs * ((rows + 255) / 256);
+    bool halves = wgs <= 2 * dev->compute_units && longest > 128, rows64 = halves && 4 * wgs64 <= 5 * dev->compute_units;
+    int v = rows64 ? 0 : halves ? 1 : 2;
+    if (getenv("XV")) v = atoi(getenv("XV"));
+    pp_parts(dev, a.c, v == 0 ? wgs64 : v >= 3 ? wgs256 : wgs, longest, 512, &a);
+#define FH_V(D) v == 0 ? pp_tiles<T, D, 2, 2, 2>(dev, a) : v == 1 ? pp_tiles<T, D, 2, 4, 2>(dev, a) : v == 2 ? pp_tiles<T, D, 1, 4, 2>(dev, a) : v == 3 ? pp_tiles<T, D, 1, 8, 2>(dev, a) : v == 4 ? pp_tiles<T, D, 1, 8, 3>(dev, a) : pp_tiles<T, D, 1, 8, 4>(dev, a)
+    if (a.c.d == 128) return FH_V(128);
+    return FH_V(64);
 }
 fh_status fh_paged_prompt(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len) {
     FH_REQUIRE((int64_t)call.rows.max_new * (call.hq / call.hkv) <= 65535LL * 64, "%d new rows of a sequence with %d heads a KV head", call.rows.max_new,
