@@ -14,7 +14,6 @@
 // what it sees (pp_again): one at a time by a wavefront, slow, and never entered by finite caches.
 #include "fh_attention_tiles.h"
 #include "fh_paged.h"
-#include <stdlib.h>
 #include <type_traits>
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
@@ -25,11 +24,26 @@ template <> struct PpVec<fh_bf> { typedef bf8 type; };
 __device__ __forceinline__ floatx16 pp_mfma(half8 a, half8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ floatx16 pp_mfma(bf8 a, bf8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
+enum { PP_PARTS = 256 }; // at most
 struct PpArgs {
     PagedCall c;
-    int parts;
+    int parts, sorted; // sorted: the longest sequences first
     float *sums, *stats; // [part][row][head][d], [part][row][head][maximum, sum]
 };
+
+// The sequence that the z-th place of the grid has: with more workgroups than run at once, and up to 64 sequences, the z-th longest, so that the short ones
+// fill what the long ones leave (8 sequences of 1.4 to 4.5 thousand positions, 184 to 512 new ones, bf16, 32 / 8 heads of 128: 202 us as they come, 188 so).
+__device__ __forceinline__ int pp_sequence(const PpArgs &a, int z) {
+    const int n = a.c.rows.seqs, lane = threadIdx.x & 63;
+    if (!a.sorted || n == 1 || n > 64) return z;
+    const int len = lane < n ? a.c.rows.lens[lane] : 0;
+    int rank = lane < n ? 0 : 64;
+    for (int j = 0; j < n; j++) {
+        const int other = __builtin_amdgcn_readlane(len, j);
+        rank += other > len || (other == len && j < lane);
+    }
+    return __builtin_amdgcn_readfirstlane(__ffsll(__ballot(rank == z)) - 1);
+}
 
 // A lane's query and what it sees: positions low .. high, if any.
 struct PpRow {
@@ -148,9 +162,9 @@ __device__ __forceinline__ void pp_check(const PpArgs &a, int part, int seq, con
 // ---------------------------------------------------------------- rows and pages of one 16-bit type, head_dim 64 or 128
 // k_attn_ahead's loop (fh_attention_prefill.hip): the scores of the next tile beside the softmax of this one, K a tile ahead of V, both straight
 // into LDS with their 16-byte pieces swapped on the memory side.
-// NB buffers: step `it` asks for K of step it + NB and V of step it + NB - 1.
-template <typename T, int D, int KS, int QW, int NB>
-__global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW >= 4 ? 2 : 1, 2))) void k_paged_tiles(PpArgs a) {
+template <typename T, int D, int KS>
+__global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_paged_tiles(PpArgs a) {
+    constexpr int QW = 4, NB = 2; // wavefronts of rows; buffers: step `it` asks for K of step it + NB and V of step it + NB - 1
     constexpr int BN = 64, DT = D / 32, KSTEPS = D / 16, CH = D / 8, TILE = BN * D, NW = QW * KS, NP = TILE * KS * 2 / 1024 / NW; // NP: 1 KB pieces of K a wavefront
     constexpr bool F16 = __is_same(T, fh_half);
     typedef typename PpVec<T>::type vec8;
@@ -159,7 +173,7 @@ __global__ __launch_bounds__(64 * QW * KS) __attribute__((amdgpu_waves_per_eu(QW
     const int kset = KS == 2 ? wave / QW : 0;
     const PagedKv &kv = a.c.kv;
     const PagedRows &rows = a.c.rows;
-    const int kh = blockIdx.x, group = a.c.hq / a.c.hkv, seq = (int)blockIdx.z / a.parts, part = (int)blockIdx.z % a.parts;
+    const int kh = blockIdx.x, group = a.c.hq / a.c.hkv, seq = pp_sequence(a, (int)blockIdx.z / a.parts), part = (int)blockIdx.z % a.parts;
     const PagedSeq s = paged_seq_scalar(rows, kv.shift, seq);
     const int r0 = (int)(gridDim.y - 1 - blockIdx.y) * 32 * QW;
     if (r0 >= s.rows * group) return;
@@ -417,7 +431,7 @@ __global__ __launch_bounds__(256) void k_paged_planes(PpArgs a) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, li = lane & 31, g = lane >> 5;
     const PagedKv &kv = a.c.kv;
     const PagedRows &rows = a.c.rows;
-    const int kh = blockIdx.x, group = a.c.hq / a.c.hkv, seq = (int)blockIdx.z / a.parts, part = (int)blockIdx.z % a.parts;
+    const int kh = blockIdx.x, group = a.c.hq / a.c.hkv, seq = pp_sequence(a, (int)blockIdx.z / a.parts), part = (int)blockIdx.z % a.parts;
     const PagedSeq s = paged_seq_scalar(rows, kv.shift, seq);
     const int r0 = (int)(gridDim.y - 1 - blockIdx.y) * 128;
     if (r0 >= s.rows * group) return;
@@ -609,27 +623,49 @@ __global__ __launch_bounds__(256) void k_paged_planes(PpArgs a) {
     pp_check<TX, TP, DP>(a, part, seq, s, r0 + wave * 32, s.rows * group, kh, group, span.base, span.base + span.steps * BN - 1, l_run, acc);
 }
 
-// ---------------------------------------------------------------- the parts together: a wavefront a row and head
+// ---------------------------------------------------------------- the parts together
+// A wavefront a row and head: lanes weigh a part each, then groups of them take parts in turn, four values a lane, eight parts on their way.
 template <typename TX>
 __global__ __launch_bounds__(256) void k_paged_join(PpArgs a) {
-    const int lane = threadIdx.x & 63, i = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
+    __shared__ float s_w[4][PP_PARTS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = (int)blockIdx.x * 4 + wave, d = a.c.d, parts = a.parts;
     const PagedSeq s = paged_seq(a.c.rows, a.c.kv.shift, blockIdx.y);
     if (i >= s.rows * a.c.hq) return;
     const int64_t row = (int64_t)s.row * a.c.hq + i, all = (int64_t)a.c.rows.tokens * a.c.hq;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < a.parts; p++) m = fmaxf(m, a.stats[2 * (p * all + row)]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    for (int p = 0; p < a.parts; p++) {
-        const float f = __builtin_amdgcn_exp2f(a.stats[2 * (p * all + row)] - ref);
-        l = fmaf(a.stats[2 * (p * all + row) + 1], f, l);
+    float m[PP_PARTS / 64], l[PP_PARTS / 64], mx = -INFINITY, den = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (lane + 64 * e < a.c.d) o[e] = fmaf(a.sums[(p * all + row) * a.c.d + lane + 64 * e], f, o[e]);
+    for (int k = 0; k < PP_PARTS / 64; k++) {
+        const int p = lane + 64 * k;
+        m[k] = -INFINITY, l[k] = 0.f;
+        if (p < parts) m[k] = a.stats[2 * (p * all + row)], l[k] = a.stats[2 * (p * all + row) + 1];
+        mx = fmaxf(mx, m[k]);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-        if (lane + 64 * e < a.c.d) ((TX *)a.c.out)[row * a.c.d + lane + 64 * e] = (TX)(o[e] * inv);
+    for (int w = 32; w; w >>= 1) mx = fmaxf(mx, __shfl_xor(mx, w));
+    const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+    for (int k = 0; k < PP_PARTS / 64; k++) {
+        const float f = __builtin_amdgcn_exp2f(m[k] - ref);
+        s_w[wave][lane + 64 * k] = f; // (read by this wavefront alone: its LDS operations are in order)
+        den = fmaf(l[k], f, den);
+    }
+#pragma unroll
+    for (int w = 32; w; w >>= 1) den += __shfl_xor(den, w);
+    int wide = 2; // lanes of a group: a power of two that has all of the row
+    while (4 * wide < d) wide *= 2;
+    const int at = lane % wide * 4, first = lane / wide, groups = 64 / wide;
+    const bool mine = at < d;
+    const float *from = a.sums + row * d + (mine ? at : 0);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int p = first; p < parts; p += groups) {
+        const float4 y = *(const float4 *)(from + p * all * d);
+        const float f = s_w[wave][p];
+        x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
+    }
+    for (int w = wide; w < 64; w *= 2) x.x += __shfl_xor(x.x, w), x.y += __shfl_xor(x.y, w), x.z += __shfl_xor(x.z, w), x.w += __shfl_xor(x.w, w);
+    const float inv = den == 0.f ? 0.f : 1.f / den; // (a row that sees nothing: zeros)
+    if (mine && first == 0) ap_store4((TX *)a.c.out + row * d + at, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
 }
 
 // ---------------------------------------------------------------- which form
@@ -637,7 +673,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PpArgs a) {
 static int pp_parts(fh_device *dev, const PagedCall &call, int64_t wgs, int64_t longest, int least, PpArgs *a) {
     int parts = (int)(dev->compute_units / wgs);
     parts = (int)(longest / least < parts ? longest / least : parts);
-    parts = parts < 1 ? 1 : parts;
+    parts = parts < 1 ? 1 : parts > PP_PARTS ? PP_PARTS : parts;
     a->parts = parts;
     if (parts == 1) return 1;
     const size_t n = (size_t)parts * call.rows.tokens * call.hq;
@@ -653,13 +689,13 @@ template <typename TX> static fh_status pp_join(fh_device *dev, const PpArgs &a)
     return FH_OK;
 }
 
-template <typename T, int D, int KS, int QW, int NB>
+template <typename T, int D, int KS>
 static fh_status pp_tiles(fh_device *dev, PpArgs a) {
-    constexpr int LDS = NB * 2 * KS * 64 * D * 2, MERGE = KS == 2 ? (2 + D / 2) * 64 * QW * 4 : 0, BYTES = LDS > MERGE ? LDS : MERGE;
-    const auto kern = k_paged_tiles<T, D, KS, QW, NB>;
+    constexpr int LDS = 4 * KS * 64 * D * 2, MERGE = KS == 2 ? (2 + D / 2) * 256 * 4 : 0, BYTES = LDS > MERGE ? LDS : MERGE;
+    const auto kern = k_paged_tiles<T, D, KS>;
     FH_TRY(fh_kernel_lds(dev, (const void *)kern, BYTES));
-    const unsigned blocks = (unsigned)(((int64_t)a.c.rows.max_new * (a.c.hq / a.c.hkv) + 32 * QW - 1) / (32 * QW));
-    kern<<<dim3((unsigned)a.c.hkv, blocks, (unsigned)(a.c.rows.seqs * a.parts)), dim3(64 * QW * KS), BYTES, dev->stream>>>(a);
+    const unsigned blocks = (unsigned)(((int64_t)a.c.rows.max_new * (a.c.hq / a.c.hkv) + 127) / 128);
+    kern<<<dim3((unsigned)a.c.hkv, blocks, (unsigned)(a.c.rows.seqs * a.parts)), dim3(256 * KS), BYTES, dev->stream>>>(a);
     FH_HIP(hipGetLastError());
     return pp_join<T>(dev, a);
 }
@@ -667,6 +703,7 @@ template <typename TX, typename TP, int DP>
 static fh_status pp_planes(fh_device *dev, PpArgs a, int64_t longest) {
     constexpr int KP = sizeof(TP) == 4 ? 3 : 1, LDS = KP * 32 * (DP + 8 + DP + 32) * 2;
     const int64_t blocks = ((int64_t)a.c.rows.max_new * (a.c.hq / a.c.hkv) + 127) / 128;
+    a.sorted = blocks * a.c.hkv * a.c.rows.seqs > dev->compute_units;
     pp_parts(dev, a.c, blocks * a.c.hkv * a.c.rows.seqs, longest, 256, &a);
     const auto kern = k_paged_planes<TX, TP, DP>;
     FH_TRY(fh_kernel_lds(dev, (const void *)kern, LDS));
@@ -682,14 +719,12 @@ template <typename TX, typename TP> static fh_status pp_dim(fh_device *dev, cons
 template <typename T> static fh_status pp_same(fh_device *dev, PpArgs a, int64_t longest) {
     if (a.c.d != 64 && a.c.d != 128) return pp_dim<T, T>(dev, a, longest);
     const int64_t rows = (int64_t)a.c.rows.max_new * (a.c.hq / a.c.hkv), pairs = (int64_t)a.c.hkv * a.c.rows.seqs;
-    const int64_t wgs = pairs * ((rows + 127) / 128), wgs64 = pairs * ((rows + 63) / 64), wgs256 = pairs * ((rows + 255) / 256);
-    bool halves = wgs <= 2 * dev->compute_units && longest > 128, rows64 = halves && 4 * wgs64 <= 5 * dev->compute_units;
-    int v = rows64 ? 0 : halves ? 1 : 2;
-    if (getenv("XV")) v = atoi(getenv("XV"));
-    pp_parts(dev, a.c, v == 0 ? wgs64 : v >= 3 ? wgs256 : wgs, longest, 512, &a);
-#define FH_V(D) v == 0 ? pp_tiles<T, D, 2, 2, 2>(dev, a) : v == 1 ? pp_tiles<T, D, 2, 4, 2>(dev, a) : v == 2 ? pp_tiles<T, D, 1, 4, 2>(dev, a) : v == 3 ? pp_tiles<T, D, 1, 8, 2>(dev, a) : v == 4 ? pp_tiles<T, D, 1, 8, 3>(dev, a) : pp_tiles<T, D, 1, 8, 4>(dev, a)
-    if (a.c.d == 128) return FH_V(128);
-    return FH_V(64);
+    const int64_t wgs = pairs * ((rows + 127) / 128);
+    const bool halves = wgs <= 2 * dev->compute_units && longest > 128;
+    a.sorted = wgs > dev->compute_units;
+    pp_parts(dev, a.c, wgs, longest, 512, &a);
+    if (a.c.d == 128) return halves ? pp_tiles<T, 128, 2>(dev, a) : pp_tiles<T, 128, 1>(dev, a);
+    return halves ? pp_tiles<T, 64, 2>(dev, a) : pp_tiles<T, 64, 1>(dev, a);
 }
 fh_status fh_paged_prompt(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len) {
     FH_REQUIRE((int64_t)call.rows.max_new * (call.hq / call.hkv) <= 65535LL * 64, "%d new rows of a sequence with %d heads a KV head", call.rows.max_new,
