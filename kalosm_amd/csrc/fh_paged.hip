@@ -57,53 +57,168 @@ enum { PAGED_AXES = 4 };
 struct PagedTurn {
     const float *cos, *sin; // [table_rows][pairs of the tables' rows]
     const int *positions;   // [axes][tokens], NULL: the position in the cache
-    int table_rows, table_pairs, pairs, axes, end[PAGED_AXES]; // pairs that turn (the first 2 * pairs of a head's values); the axis' last pair + 1
+    int table_rows, table_pairs, pairs, axes, aligned, end[PAGED_AXES]; // aligned: four of a row's pairs are 16 bytes; pairs that turn (the first 2 * pairs of a head's values); the axis' last pair + 1
 };
 
-// One workgroup a row; a thread takes the pairs and the values of all heads in turn.
+// Where a row goes: its sequence's page and slot, and its positions on the axes; at < 0: nowhere.  By scalar loads: a search through the starts
+// (of few sequences: all in one cache line), the length and the axes' positions, the table.
+struct PagedPlace {
+    int64_t at; // bytes into the pages of head 0
+    int where0, where1, where2, where3;
+};
+__device__ __forceinline__ PagedPlace paged_place(int row, const PagedRows &rows, const PagedKv &kv, const PagedTurn &turn) {
+    PagedPlace x = {-1, 0, 0, 0, 0};
+    const int *given = turn.positions ? turn.positions + row : rows.lens; // (axes that there are not: the first one's again)
+    const int t = rows.tokens, g0 = paged_scalar(given, 0), g1 = paged_scalar(given, turn.positions && turn.axes > 1 ? t : 0),
+              g2 = paged_scalar(given, turn.positions && turn.axes > 2 ? 2 * (int64_t)t : 0), g3 = paged_scalar(given, turn.positions && turn.axes > 3 ? 3 * (int64_t)t : 0);
+    int seq = row, p;
+    if (!rows.starts) p = paged_scalar(rows.lens, row) - 1;
+    else {
+        int lo = 0, hi = rows.seqs; // the last sequence that begins at or before the row
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (paged_scalar(rows.starts, mid) <= row) lo = mid;
+            else hi = mid;
+        }
+        const int begin = paged_scalar(rows.starts, lo), end = paged_scalar(rows.starts, lo + 1), len = paged_scalar(rows.lens, lo);
+        if (row < begin || row >= end) return x; // before the first or behind the last sequence
+        seq = lo, p = len > FH_PAGED_MAX ? -1 : len - (end - row);
+    }
+    if (p < 0 || p >> kv.shift >= rows.cols) return x;
+    const int page = paged_scalar(rows.table, (int64_t)seq * rows.cols + (p >> kv.shift));
+    x.where0 = x.where1 = x.where2 = x.where3 = p;
+    if (turn.positions) x.where0 = g0, x.where1 = g1, x.where2 = g2, x.where3 = g3;
+    const unsigned end = (unsigned)turn.table_rows;
+    const bool fits = !turn.pairs || ((unsigned)x.where0 < end && (unsigned)x.where1 < end && (unsigned)x.where2 < end && (unsigned)x.where3 < end);
+    if (fits && (unsigned)page < (unsigned)kv.pages) x.at = page * kv.page + (p & ((1 << kv.shift) - 1)) * kv.slot;
+    return x;
+}
+__device__ __forceinline__ int paged_axis_position(const PagedTurn &turn, const PagedPlace &x, int pair) {
+    const int p0 = x.where0, p1 = x.where1, p2 = x.where2, p3 = x.where3; // (values: a choice among a structure's fields would put it into LDS)
+    const int p = pair >= turn.end[0] ? p1 : p0, r = pair >= turn.end[1] ? p2 : p;
+    return pair >= turn.end[2] ? p3 : r;
+}
+
+// Eight values of a row in memory.
+template <typename T> struct Paged8 {
+    T v[8];
+};
+template <typename T> __device__ __forceinline__ Paged8<T> paged_load8(const T *p) { // at a multiple of 16 bytes
+    Paged8<T> x;
+    const uint4 *u = (const uint4 *)p;
+    uint4 w[sizeof(T) / 2];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = u[i];
+    __builtin_memcpy(&x, w, sizeof(x));
+    return x;
+}
+template <typename T> __device__ __forceinline__ void paged_store8(T *p, const float (&y)[8]) {
+    T v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = (T)y[e];
+    uint4 w[sizeof(T) / 2];
+    __builtin_memcpy(w, v, sizeof(v));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) ((uint4 *)p)[i] = w[i];
+}
+
+// A thread takes eight pairs of a head, or eight values that are copied (V, what the sections leave): moves 4 to 6 bytes an operation, so it is bound by the
+// memory for many rows, and by the chain of requests for few: the values are asked for before the row's place is looked up.
+// grid (rows, units of a row / 256)
+template <typename TX, typename TP, bool TANGLED>
+__global__ __launch_bounds__(256) void k_paged_append8(const TX *q, const TX *__restrict__ k, const TX *__restrict__ v, int hq, int hkv, int d, int n,
+                                                       const int *__restrict__ starts, const int *__restrict__ lens, int seqs, int cols, int64_t q_st, int64_t q_sh,
+                                                       int64_t kv_st, int64_t kv_sh, const int *__restrict__ table, int tokens, PagedKv kv, PagedTurn turn,
+                                                       TX *q_out) { // (q_out may be q)
+    const PagedRows rows = {starts, lens, table, cols, seqs, tokens, 0};
+    const int row = blockIdx.x;
+    int u = (int)blockIdx.y * 256 + threadIdx.x;
+    const int heads = hq + hkv, turns = n / 8, copies = (d - 2 * n) / 8; // of a head (hq: 0 without q)
+    // which of the row's units: pairs of q and k, then what is copied of them, then V (threads behind the last: that one, and they store nothing)
+    const int all = heads * (turns + copies) + hkv * (d / 8);
+    const bool mine = u < all;
+    u = mine ? u : all - 1;
+    int h, a, b; // head of q and k together (V: heads ..), its values a .. and b ..
+    const bool turned = u < heads * turns;
+    if (turned) {
+        h = u / turns, a = (u - h * turns) * 8;
+        if (TANGLED) a *= 2, b = a + 8;
+        else b = a + n;
+    } else if ((u -= heads * turns) < heads * copies) h = u / copies, a = b = 2 * n + (u - h * copies) * 8;
+    else u -= heads * copies, h = u / (d / 8), a = b = (u - h * (d / 8)) * 8, h += heads;
+    const TX *base = h < hq ? q : h < heads ? k : v;
+    const int64_t st = h < hq ? q_st : kv_st, off = h < hq ? h * q_sh : (h - (h < heads ? hq : heads)) * kv_sh;
+    const Paged8<TX> x = paged_load8(base + row * st + off + a), y = paged_load8(base + row * st + off + b);
+    const PagedPlace to = paged_place(row, rows, kv, turn);
+    if (to.at < 0 || !mine) return;
+    float p[8], r[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) p[e] = (float)x.v[e], r[e] = (float)y.v[e];
+    if (turned) {
+        const int j = TANGLED ? a / 2 : a; // first pair
+        bool one = turn.aligned; // axis for all eight
+#pragma unroll
+        for (int e = 0; e + 1 < PAGED_AXES; e++) one &= j >= turn.end[e] || j + 7 < turn.end[e];
+        float c[8], s[8];
+        if (one) {
+            const int64_t at = (int64_t)paged_axis_position(turn, to, j) * turn.table_pairs + j;
+            const float4 c0 = *(const float4 *)(turn.cos + at), c1 = *(const float4 *)(turn.cos + at + 4), s0 = *(const float4 *)(turn.sin + at), s1 = *(const float4 *)(turn.sin + at + 4);
+            c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
+            s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
+        } else
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int64_t at = (int64_t)paged_axis_position(turn, to, j + e) * turn.table_pairs + j + e;
+                c[e] = turn.cos[at], s[e] = turn.sin[at];
+            }
+        if (TANGLED) {
+            float z[16];
+#pragma unroll
+            for (int e = 0; e < 8; e++) z[e] = p[e], z[8 + e] = r[e];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float f = z[2 * e], g = z[2 * e + 1];
+                z[2 * e] = f * c[e] - g * s[e], z[2 * e + 1] = f * s[e] + g * c[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) p[e] = z[e], r[e] = z[8 + e];
+        } else
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float f = p[e], g = r[e];
+                p[e] = f * c[e] - g * s[e], r[e] = f * s[e] + g * c[e];
+            }
+    }
+    if (h < hq) {
+        TX *o = q_out + ((int64_t)row * hq + h) * d;
+        paged_store8(o + a, p);
+        if (turned) paged_store8(o + b, r);
+    } else {
+        TP *o = (TP *)((char *)(h < heads ? kv.k : kv.v) + to.at + (h < heads ? h - hq : h - heads) * kv.head);
+        paged_store8(o + a, p);
+        if (turned) paged_store8(o + b, r);
+    }
+}
+
+// The same a value or pair at a time, for rows that do not begin at multiples of 16 bytes and pairs that are no multiple of eight.  One workgroup a row.
 template <typename TX, typename TP, bool TANGLED>
 __global__ __launch_bounds__(256) void k_paged_append(const TX *q, int64_t q_st, int64_t q_sh, const TX *__restrict__ k, const TX *__restrict__ v,
                                                       int64_t kv_st, int64_t kv_sh, int hq, int hkv, int d, PagedTurn turn, PagedKv kv, PagedRows rows,
                                                       TX *q_out) { // (q_out may be q)
     const int row = blockIdx.x, tid = threadIdx.x;
-    int lo = 0, hi = rows.seqs; // the sequence whose rows this one is among: the last that begins at or before it
-    if (rows.starts)
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (rows.starts[mid] <= row) lo = mid;
-            else hi = mid;
-        }
-    else
-        lo = row;
-    if (rows.starts && (row < rows.starts[lo] || row >= rows.starts[lo + 1])) return; // before the first or behind the last sequence
-    const int len = rows.lens[lo], p = rows.starts ? len - (rows.starts[lo + 1] - row) : len - 1;
-    if (len > FH_PAGED_MAX || p < 0 || p >> kv.shift >= rows.cols) return;
-    const int page = rows.table[(int64_t)lo * rows.cols + (p >> kv.shift)];
-    if ((unsigned)page >= (unsigned)kv.pages) return;
-    const int64_t at = (int64_t)page * kv.page + (int64_t)(p & ((1 << kv.shift) - 1)) * kv.slot;
-    int where[PAGED_AXES] = {p, p, p, p};
-    if (turn.pairs) {
-        for (int a = 0; a < turn.axes; a++) {
-            if (turn.positions) where[a] = turn.positions[(int64_t)a * rows.tokens + row];
-            if ((unsigned)where[a] >= (unsigned)turn.table_rows) return;
-        }
-    }
-    const int units = d / 2, turned = (q ? hq : 0) + hkv;
-    for (int i = tid; i < turned * units; i += 256) {
-        const int h = i / units, j = i % units;
-        const bool is_q = q && h < hq;
-        const int kh = h - (q ? hq : 0);
+    const PagedPlace place = paged_place(row, rows, kv, turn);
+    if (place.at < 0) return;
+    const int units = d / 2;
+    for (int i = tid; i < (hq + hkv) * units; i += 256) {
+        const int h = i / units, j = i % units, kh = h - hq;
+        const bool is_q = h < hq;
         const TX *from = is_q ? q + row * q_st + h * q_sh : k + row * kv_st + kh * kv_sh;
         int a = 2 * j, b = 2 * j + 1; // behind the turned pairs: neighbours, as they are
         float c = 1.f, s = 0.f;
         if (j < turn.pairs) {
             if (!TANGLED) a = j, b = j + turn.pairs;
-            int pos = where[0];
-#pragma unroll
-            for (int e = 0; e + 1 < PAGED_AXES; e++)
-                if (j >= turn.end[e]) pos = where[e + 1];
-            c = turn.cos[(int64_t)pos * turn.table_pairs + j];
-            s = turn.sin[(int64_t)pos * turn.table_pairs + j];
+            const int64_t at = (int64_t)paged_axis_position(turn, place, j) * turn.table_pairs + j;
+            c = turn.cos[at], s = turn.sin[at];
         }
         const float x = (float)from[a], y = (float)from[b];
         const float u = j < turn.pairs ? x * c - y * s : x, w = j < turn.pairs ? x * s + y * c : y;
@@ -111,13 +226,13 @@ __global__ __launch_bounds__(256) void k_paged_append(const TX *q, int64_t q_st,
             TX *to = q_out + ((int64_t)row * hq + h) * d;
             to[a] = (TX)u, to[b] = (TX)w;
         } else {
-            TP *to = (TP *)((char *)kv.k + at + kh * kv.head);
+            TP *to = (TP *)((char *)kv.k + place.at + kh * kv.head);
             to[a] = (TP)u, to[b] = (TP)w;
         }
     }
     for (int i = tid; i < hkv * d; i += 256) {
         const int h = i / d, e = i % d;
-        ((TP *)((char *)kv.v + at + h * kv.head))[e] = (TP)v[row * kv_st + h * kv_sh + e];
+        ((TP *)((char *)kv.v + place.at + h * kv.head))[e] = (TP)v[row * kv_st + h * kv_sh + e];
     }
 }
 
@@ -153,15 +268,29 @@ extern "C" fh_status fh_paged_rope_append(fh_device *dev, int32_t dtype, int32_t
         FH_REQUIRE(n > 0, "sections without a pair");
         turn.cos = cos_dev, turn.sin = sin_dev, turn.positions = positions_dev;
         turn.table_rows = table_rows, turn.table_pairs = table_pairs, turn.pairs = (int)n, turn.axes = axes;
+        turn.aligned = !(((uintptr_t)cos_dev | (uintptr_t)sin_dev) & 15) && table_pairs % 4 == 0;
     } else
         FH_REQUIRE(!positions_dev && !sections_host, "positions without tables");
     FH_REQUIRE(dev, "NULL device");
     if (!tokens || !seqs) return FH_OK;
     PagedGpu gpu;
     FH_TRY(gpu.enter(dev));
-#define FH_PA(TX, TP)                                                                                                                            \
-    (interleaved ? k_paged_append<TX, TP, true> : k_paged_append<TX, TP, false>)<<<dim3((unsigned)tokens), dim3(256), 0, dev->stream>>>(            \
-        (const TX *)q_dev, q_st, q_sh, (const TX *)k_dev, (const TX *)v_dev, kv_st, kv_sh, hq, hkv, d, turn, kv, rows, (TX *)q_out_dev)
+    const int size = dtype == FH_F32 ? 4 : 2, heads = q_dev ? hq : 0;
+    auto odd = [&](const void *p, int64_t st, int64_t sh) { return ((uintptr_t)p | (uintptr_t)(st * size) | (uintptr_t)(sh * size)) & 15; };
+    const bool eights = turn.pairs % 8 == 0 && !(q_dev && (odd(q_dev, q_st, q_sh) || odd(q_out_dev, 0, 0))) && !odd(k_dev, kv_st, kv_sh) && !odd(v_dev, kv_st, kv_sh);
+    const int64_t units = (int64_t)(heads + hkv) * (turn.pairs / 8 + (d - 2 * turn.pairs) / 8) + (int64_t)hkv * (d / 8);
+    const dim3 grid((unsigned)tokens, eights ? (unsigned)((units + 255) / 256) : 1u), block(256);
+#define FH_PA(TX, TP)                                                                                                                              \
+    do {                                                                                                                                           \
+        const TX *q = (const TX *)q_dev, *k = (const TX *)k_dev, *v = (const TX *)v_dev;                                                           \
+        if (eights)                                                                                                                                \
+            (interleaved ? k_paged_append8<TX, TP, true> : k_paged_append8<TX, TP, false>)<<<grid, block, 0, dev->stream>>>(                       \
+                q, k, v, heads, hkv, d, turn.pairs, starts_dev, lens_dev, seqs, table_cols, q_st, q_sh, kv_st, kv_sh, table_dev, tokens, kv, turn, \
+                (TX *)q_out_dev);                                                                                                                  \
+        else                                                                                                                                       \
+            (interleaved ? k_paged_append<TX, TP, true> : k_paged_append<TX, TP, false>)<<<grid, block, 0, dev->stream>>>(                         \
+                q, q_st, q_sh, k, v, kv_st, kv_sh, heads, hkv, d, turn, kv, rows, (TX *)q_out_dev);                                                \
+    } while (0)
     if (dtype == FH_F16) FH_PA(fh_half, fh_half);
     else if (dtype == FH_PAGED_BF16) FH_PA(fh_bf, fh_bf);
     else if (kv_dtype == FH_F32) FH_PA(float, float);
