@@ -44,6 +44,49 @@ __device__ __forceinline__ PagedSeq paged_seq_scalar(const PagedRows &r, int shi
     return r.starts ? paged_seq(r, shift, len, paged_scalar(r.starts, i), paged_scalar(r.starts, i + 1)) : paged_seq(r, shift, len, i, i + 1);
 }
 
+// One row and head by a wavefront, over the positions from .. to: what the tiles are checked against where they end up infinite or NaN (an infinity or a NaN
+// among values that a neighbour sees and this row does not, terms of an infinite f32).  A key a lane for the scores; o[e]: value lane + 64 e.  m is in
+// the log2 domain, weights are 2^shift times what they are.
+template <typename TX, typename TP>
+__device__ __forceinline__ void paged_again(const TX *q, int d, float sc2, float shift, const PagedKv &kv, const int *table, int kh, int from, int to, float &m, float &l,
+                                            float (&o)[4]) {
+    const int lane = threadIdx.x & 63;
+    m = -INFINITY, l = 0.f;
+    for (int e = 0; e < 4; e++) o[e] = 0.f;
+    for (int t = from; t <= to; t += 64) {
+        const int key = t + lane;
+        float y = -INFINITY;
+        int64_t at = -1;
+        if (key <= to) {
+            const int page = table[key >> kv.shift];
+            if ((unsigned)page < (unsigned)kv.pages) {
+                at = page * kv.page + kh * kv.head + (key & ((1 << kv.shift) - 1)) * kv.slot;
+                y = 0.f;
+#pragma unroll 1
+                for (int e = 0; e < d; e++) y = fmaf((float)q[e], (float)((const TP *)(kv.k + at))[e], y);
+                y *= sc2;
+            }
+        }
+        float mx = y;
+        for (int w = 32; w; w >>= 1) mx = fmaxf(mx, __shfl_xor(mx, w));
+        mx = fmaxf(mx, m);
+        const float ref = mx == -INFINITY ? 0.f : mx, alpha = __builtin_amdgcn_exp2f(m - ref), pr = at < 0 ? 0.f : __builtin_amdgcn_exp2f(y - ref + shift);
+        m = mx;
+        float sum = pr;
+        for (int w = 32; w; w >>= 1) sum += __shfl_xor(sum, w);
+        l = l * alpha + sum;
+        for (int e = 0; e < 4; e++) o[e] *= alpha;
+#pragma unroll 1 // (few registers: it stands behind loops that have none left)
+        for (int j = 0; j < 64; j++) {
+            const int64_t v = __shfl(at, j);
+            const float p = __shfl(pr, j);
+            if (v >= 0)
+                for (int e = 0; e < 4; e++)
+                    if (lane + 64 * e < d) o[e] = fmaf(p, (float)((const TP *)(kv.v + v))[lane + 64 * e], o[e]);
+        }
+    }
+}
+
 // Arguments both entry points check, without touching a device: FH_OK, or an error with its message.  `kv` and `rows` are filled in.
 fh_status fh_paged_arguments(int dtype, int kv_dtype, int hq, int hkv, int d, const void *k_pages, const void *v_pages, int64_t page_stride,
                              int64_t head_stride, int64_t slot_stride, int pages, int page_size, const int32_t *starts, const int32_t *lens,
@@ -58,7 +101,7 @@ struct PagedCall {
     float scale;
     int window, hq, hkv, d;
 };
-fh_status fh_paged_step(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len); // rows.max_new = 1
+fh_status fh_paged_step(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len); // rows.max_new rows of all heads of a KV head: 16 at most, or one row
 fh_status fh_paged_prompt(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len);
 // The GPU of `dev` is the calling thread's current one while this lives.
 struct PagedGpu {

@@ -320,6 +320,6 @@ extern "C" fh_status fh_paged_attention(fh_device *dev, int32_t dtype, int32_t k
     PagedGpu gpu;
     FH_TRY(gpu.enter(dev));
     const PagedCall call = {q_dev, out_dev, q_st, q_sh, kv, rows, scale, window, hq, hkv, d};
-    if (rows.max_new == 1) return fh_paged_step(dev, dtype, kv_dtype, call, max_len);
+    if (rows.max_new == 1 || (int64_t)rows.max_new * (hq / hkv) <= 16) return fh_paged_step(dev, dtype, kv_dtype, call, max_len);
     return fh_paged_prompt(dev, dtype, kv_dtype, call, max_len);
 }

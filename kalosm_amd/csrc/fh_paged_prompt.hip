@@ -93,46 +93,15 @@ __device__ __forceinline__ void pp_store(const PpArgs &a, int part, const PagedS
     }
 }
 
-// Row r of a sequence again, positions from .. to of those that it sees: a key a lane for the scores, values lane, lane + 64 .. for the sums.
+// Row r of a sequence again, positions from .. to of those that it sees.
 template <typename TX, typename TP>
 __device__ __forceinline__ void pp_again(const PpArgs &a, int part, int seq, const PagedSeq &s, int r, int kh, int group, int from, int to) {
-    const PagedKv &kv = a.c.kv;
     const int lane = threadIdx.x & 63, d = a.c.d;
     const PpRow x = pp_row(s, r, group, a.c.window);
-    from = from > x.low ? from : x.low, to = to < x.high ? to : x.high;
     const TX *q = (const TX *)a.c.q + (s.row + x.token) * a.c.q_st + (kh * group + x.head) * a.c.q_sh;
-    const float sc2 = a.c.scale * 1.4426950408889634f, shift = __is_same(TP, fh_half) ? 14.f : 0.f;
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int t = from; t <= to; t += 64) {
-        const int key = t + lane;
-        float y = -INFINITY;
-        int64_t at = -1;
-        if (key <= to) {
-            const int page = a.c.rows.table[(int64_t)seq * a.c.rows.cols + (key >> kv.shift)];
-            if ((unsigned)page < (unsigned)kv.pages) {
-                at = page * kv.page + kh * kv.head + (key & ((1 << kv.shift) - 1)) * kv.slot;
-                y = 0.f;
-                for (int e = 0; e < d; e++) y = fmaf((float)q[e], (float)((const TP *)(kv.k + at))[e], y);
-                y *= sc2;
-            }
-        }
-        float mx = y;
-        for (int w = 32; w; w >>= 1) mx = fmaxf(mx, __shfl_xor(mx, w));
-        mx = fmaxf(mx, m);
-        const float ref = mx == -INFINITY ? 0.f : mx, alpha = __builtin_amdgcn_exp2f(m - ref), pr = at < 0 ? 0.f : __builtin_amdgcn_exp2f(y - ref + shift);
-        m = mx;
-        float sum = pr;
-        for (int w = 32; w; w >>= 1) sum += __shfl_xor(sum, w);
-        l = l * alpha + sum;
-        for (int e = 0; e < 4; e++) o[e] *= alpha;
-        for (int j = 0; j < 64; j++) {
-            const int64_t v = __shfl(at, j);
-            const float p = __shfl(pr, j);
-            if (v >= 0)
-                for (int e = 0; e < 4; e++)
-                    if (lane + 64 * e < d) o[e] = fmaf(p, (float)((const TP *)(kv.v + v))[lane + 64 * e], o[e]);
-        }
-    }
+    float m, l, o[4];
+    paged_again<TX, TP>(q, d, a.c.scale * 1.4426950408889634f, __is_same(TP, fh_half) ? 14.f : 0.f, a.c.kv, a.c.rows.table + (int64_t)seq * a.c.rows.cols, kh,
+                        from > x.low ? from : x.low, to < x.high ? to : x.high, m, l, o);
     const int64_t row = (int64_t)(s.row + x.token) * a.c.hq + kh * group + x.head, where = (int64_t)part * a.c.rows.tokens * a.c.hq + row;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     for (int e = 0; e < 4; e++)
@@ -159,7 +128,7 @@ __device__ __forceinline__ void pp_check(const PpArgs &a, int part, int seq, con
         if (bad >> i & 1 && first + i < rows) pp_again<TX, TP>(a, part, seq, s, first + i, kh, group, from, to);
 }
 
-// ---------------------------------------------------------------- rows and pages of one 16-bit type, head_dim 64 or 128
+// ---------------------------------------------------------------- rows and pages of one 16-bit type, head_dim up to 128 (in tiles of 64 or 128 values)
 // k_attn_ahead's loop (fh_attention_prefill.hip): the scores of the next tile beside the softmax of this one, K a tile ahead of V, both straight
 // into LDS with their 16-byte pieces swapped on the memory side.
 template <typename T, int D, int KS>
@@ -187,7 +156,9 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(2, 2))
     constexpr int RSTEP = NW * 64 / CH;
     static_assert(RSTEP % 16 == 0 && 64 / CH <= 16, "the same swap in all of a lane's rows, one page a piece");
     const int row = (wave * 64 + lane) / CH, piece = lane % CH, slot = (int)kv.slot;
-    const int kc = (piece ^ (D == 128 ? row & 15 : (row >> 1) & 7)) * 16, vc = (piece ^ (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2)) * 16;
+    // (pieces behind the head's end: its first one again.  Q is zero there, and V's outputs are not stored)
+    auto in_head = [&](int c) { return c < a.c.d * 2 ? c : 0; };
+    const int kc = in_head((piece ^ (D == 128 ? row & 15 : (row >> 1) & 7)) * 16), vc = in_head((piece ^ (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2)) * 16);
     const int last16 = (s.len - 1) & ~15; // the last 16 positions there are
     auto begin16 = [&](int it, int i) __attribute__((always_inline)) {
         const int p = span.base + it * KS * BN + ((i * RSTEP + wave * (64 / CH)) & ~15);
@@ -253,7 +224,10 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(2, 2))
     {
         const T *qp = (const T *)a.c.q + (s.row + x.token) * a.c.q_st + (kh * group + x.head) * a.c.q_sh + 8 * g;
 #pragma unroll
-        for (int ks = 0; ks < KSTEPS; ks++) __builtin_memcpy(&qf[ks], qp + 16 * ks, 16); // (any address)
+        for (int ks = 0; ks < KSTEPS; ks++) {
+            qf[ks] = vec8{};
+            if (16 * ks + 8 * g < a.c.d) __builtin_memcpy(&qf[ks], qp + 16 * ks, 16); // (any address)
+        }
     }
     const int prow = 16 * (li >> 4) + 8 * ((li >> 2) & 1) + 4 * ((li >> 3) & 1) + (li & 3); // key read by MFMA row li
     const uint32_t k_at = kset * TILE * 2 + prow * D * 2 + (g ^ (D == 128 ? prow & 15 : (prow >> 1) & 7)) * 16; // bytes
@@ -717,13 +691,13 @@ template <typename TX, typename TP> static fh_status pp_dim(fh_device *dev, cons
     return pp_planes<TX, TP, 256>(dev, a, longest);
 }
 template <typename T> static fh_status pp_same(fh_device *dev, PpArgs a, int64_t longest) {
-    if (a.c.d != 64 && a.c.d != 128) return pp_dim<T, T>(dev, a, longest);
+    if (a.c.d > 128) return pp_planes<T, T, 256>(dev, a, longest);
     const int64_t rows = (int64_t)a.c.rows.max_new * (a.c.hq / a.c.hkv), pairs = (int64_t)a.c.hkv * a.c.rows.seqs;
     const int64_t wgs = pairs * ((rows + 127) / 128);
     const bool halves = wgs <= 2 * dev->compute_units && longest > 128;
     a.sorted = wgs > dev->compute_units;
     pp_parts(dev, a.c, wgs, longest, 512, &a);
-    if (a.c.d == 128) return halves ? pp_tiles<T, 128, 2>(dev, a) : pp_tiles<T, 128, 1>(dev, a);
+    if (a.c.d > 64) return halves ? pp_tiles<T, 128, 2>(dev, a) : pp_tiles<T, 128, 1>(dev, a);
     return halves ? pp_tiles<T, 64, 2>(dev, a) : pp_tiles<T, 64, 1>(dev, a);
 }
 fh_status fh_paged_prompt(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len) {

@@ -22,7 +22,6 @@
 // them up, in their order: the same bits in every run.  Pairs of few tiles are a workgroup each, and nothing is joined.
 #include "fh_paged.h"
 #include <type_traits>
-#include <stdlib.h>
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -65,17 +64,16 @@ __device__ __forceinline__ uint32_t ps_scan(uint32_t x) { // inclusive prefix su
 template <typename TP> struct PsVec { typedef half8 type; };
 template <> struct PsVec<fh_bf> { typedef bf8 type; };
 
-// A pair's tiles: positions first * TK .. (first + tiles) * TK - 1, of which begin .. end - 1 are seen.
+// A pair's tiles: positions first * TK .. (first + tiles) * TK - 1, of which begin .. end - 1 are seen by one of its rows, the first of which has position p.
 struct PsSpan {
-    int row, begin, end, first, tiles;
+    int row, rows, p, begin, end, first, tiles;
 };
 template <int TK> __device__ __forceinline__ PsSpan ps_span(const PagedSeq &s, int window) {
     PsSpan r;
-    r.row = s.row;
-    const int p = s.first;
-    r.end = p + 1 < s.len ? p + 1 : s.len;
+    r.row = s.row, r.rows = s.rows, r.p = s.first;
+    r.end = r.p + r.rows < s.len ? r.p + r.rows : s.len;
     r.end = r.end < 0 ? 0 : r.end;
-    r.begin = window && p - window + 1 > 0 ? p - window + 1 : 0;
+    r.begin = window && r.p - window + 1 > 0 ? r.p - window + 1 : 0;
     r.begin = r.begin < r.end ? r.begin : r.end;
     r.first = r.begin / TK;
     r.tiles = (r.end + TK - 1) / TK - r.first;
@@ -89,7 +87,7 @@ template <typename TX, typename TP, int DP, int NWV>
 __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__ table, const int *__restrict__ lens, const int *__restrict__ starts, int cols, int shift,
                                                          int whole, int hkv, int blocks, int window, int pages, const char *__restrict__ k_pages,
                                                          const char *__restrict__ v_pages, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
-                                                         const TX *__restrict__ q, int64_t q_st, int64_t q_sh, int group, int d, float scale, int seqs, int tokens, int least,
+                                                         const TX *__restrict__ q, int64_t q_st, int64_t q_sh, int group, int d, float scale, int seqs, int tokens, int max_new, int least,
                                                          int place, float *__restrict__ sums, uint32_t *__restrict__ arrived, TX *__restrict__ out) {
     constexpr bool F32 = sizeof(TP) == 4, F16 = __is_same(TP, fh_half), MIXED = sizeof(TX) != sizeof(TP);
     constexpr int TK = F32 ? 16 : 32, HALVES = TK / 16;
@@ -101,9 +99,9 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
     typedef typename PsVec<TP>::type vec8;
     extern __shared__ __attribute__((aligned(16))) float ps_lds[];
     __shared__ float s_st[NWV * 16 * 2];
-    __shared__ uint32_t s_last;
+    __shared__ uint32_t s_last, s_bad[16];
     const int tid = threadIdx.x, wave = ps_uniform(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
-    const PagedRows rows = {starts, lens, table, cols, seqs, tokens, 1};
+    const PagedRows rows = {starts, lens, table, cols, seqs, tokens, max_new};
     const int H = hkv * blocks, page_mask = (1 << shift) - 1;
 
     // ---- this workgroup's stretch of the line: `step` tiles.  Places on the line are counted from the stretch's beginning.
@@ -152,7 +150,8 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
             }
         const int in = __popcll(__ballot((before + upto) * H <= lo)); // sequences of these 64 that end before
         cur.b = ps_uniform(c + in);
-        cur.s.row = __builtin_amdgcn_readlane(mine.row, in), cur.s.begin = __builtin_amdgcn_readlane(mine.begin, in), cur.s.end = __builtin_amdgcn_readlane(mine.end, in);
+        cur.s.row = __builtin_amdgcn_readlane(mine.row, in), cur.s.rows = __builtin_amdgcn_readlane(mine.rows, in), cur.s.p = __builtin_amdgcn_readlane(mine.p, in);
+        cur.s.begin = __builtin_amdgcn_readlane(mine.begin, in), cur.s.end = __builtin_amdgcn_readlane(mine.end, in);
         cur.s.first = __builtin_amdgcn_readlane(mine.first, in), cur.s.tiles = __builtin_amdgcn_readlane(mine.tiles, in);
         const int64_t at = (before + (in ? (uint32_t)__builtin_amdgcn_readlane(upto, in - 1) : 0u)) * H - lo;
         cur.hh = (int)(-at / cur.s.tiles);
@@ -242,18 +241,25 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
 #pragma unroll
                 for (int c = 0; c < VL; c++) vr[h][j][c] = *(const vpiece *)(vb[h] + (v_off[j] + v_piece[c]));
     };
-    // Q's values of a pair as they lie: lane (head n, g) has those of K's pieces; zeros for columns without a head and behind the head's end
+    // A pair's columns are its rows' heads: column c of a sequence is head c % group of row c / group (one row: of head c).  Places 16 columns at a time.
+    auto columns = [&](const Cursor &c) { // of this block
+        const int n = c.s.rows * group - (c.hh - c.kh * blocks) * 16;
+        return n < 16 ? n : 16;
+    };
+    auto row_of = [&](int column) { return max_new == 1 ? 0 : column / group; };
+    // Q's values of a pair as they lie: lane (column n, g) has those of K's pieces; zeros for columns that there are not and behind the head's end
     constexpr int E = 16 / (int)sizeof(TP); // values of a piece
     TX rq[KL][E];
     auto ask_q = [&](const Cursor &c) {
-        const int skip = (c.hh - c.kh * blocks) * 16, head = c.kh * group + skip + n;
-        const TX *p = q + c.s.row * q_st + head * q_sh;
+        const int column = (c.hh - c.kh * blocks) * 16 + n, r = row_of(column);
+        const TX *p = q + (c.s.row + r) * q_st + (c.kh * group + column - r * group) * q_sh;
+        const bool there = n < columns(c);
 #pragma unroll
         for (int s = 0; s < KL; s++) {
             const int at = 4 * E * s + E * g;
 #pragma unroll
             for (int e = 0; e < E; e++) rq[s][e] = (TX)0.f;
-            if (skip + n < group && at < d) __builtin_memcpy(rq[s], p + at, sizeof(rq[s])); // (any address)
+            if (there && at < d) __builtin_memcpy(rq[s], p + at, sizeof(rq[s])); // (any address)
         }
     };
     ask_q(cur);
@@ -272,7 +278,11 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
     // ---- pair after pair
     bool go = true;
     while (go) {
-        const int skip = (cur.hh - cur.kh * blocks) * 16, h0 = cur.kh * group + skip, heads = group - skip < 16 ? group - skip : 16; // h0: first query head
+        const int skip = (cur.hh - cur.kh * blocks) * 16, heads = columns(cur); // (columns `skip` and up)
+        // what this lane's column sees, and what all of them see
+        const int my_p = cur.s.p + (row_of(skip + n) < cur.s.rows ? row_of(skip + n) : cur.s.rows - 1), last_p = cur.s.p + cur.s.rows - 1;
+        const int high = my_p < cur.s.end - 1 ? my_p : cur.s.end - 1, low = window && my_p - window + 1 > 0 ? my_p - window + 1 : 0;
+        const int all_high = cur.s.p < cur.s.end - 1 ? cur.s.p : cur.s.end - 1, all_low = window && last_p - window + 1 > 0 ? last_p - window + 1 : 0;
         vec8 qf[QT][F32 ? 1 : KL];
         floatx4 qx[F32 ? KL : 1];
         float sc2 = scale * 1.4426950408889634f; // scores in the log2 domain
@@ -344,15 +354,15 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
             look_up();
             __builtin_amdgcn_sched_barrier(0);
             // ---- positions that are not seen: scores -inf, values 0 (they may be anything)
-            const bool edge = first < cur.s.begin || first + TK > cur.s.end || hole;
+            const bool edge = first < all_low || first + TK - 1 > all_high || hole;
             if (edge) {
 #pragma unroll
                 for (int h = 0; h < HALVES; h++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int key = first + 16 * h + 4 * g + i;
-                        const bool seen = key >= cur.s.begin && key < cur.s.end && !(hole >> h & 1);
-                        st[h][i] = seen ? st[h][i] : -INFINITY;
+                        const bool there = !(hole >> h & 1), seen = key >= cur.s.begin && key < cur.s.end && there;
+                        st[h][i] = key >= low && key <= high && there ? st[h][i] : -INFINITY;
 #pragma unroll
                         for (int c = 0; c < VL; c++)
 #pragma unroll
@@ -423,7 +433,7 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
         // ---- the wavefronts' results together: thread (head, four values); the next pair's Q is on its way
         Cursor next = cur;
         go = next_pair(next);
-        if (go) ask_q(next);
+        if (go && !MIXED) ask_q(next); // (f32 rows over 16-bit pages: behind the merge, for want of registers)
         l_run = ps_rows_sum(l_run);
         if (n < heads) {
             float *to = ps_lds + (wave * heads + n) * DP;
@@ -437,19 +447,24 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
                             floatx4{acc[c * VE + e][i], acc[c * VE + e + 1][i], acc[c * VE + e + 2][i], acc[c * VE + e + 3][i]};
             if (g == 0) s_st[(wave * 16 + n) * 2] = m_run, s_st[(wave * 16 + n) * 2 + 1] = l_run;
         }
+        if (tid < 16) s_bad[tid] = 0;
         __syncthreads();
         const bool all = cur.from == 0 && cur.to == cur.s.tiles;
         constexpr int PITCH = DP + 4, QUADS = DP / 4; // PITCH: of a part's head: values, maximum, sum
         float *own = sums + ((int64_t)blockIdx.x * 2 + (cur.from ? 0 : 1)) * place;
         auto put = [&](float *p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
         auto get = [&](const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+        auto place_of = [&](int h) { // of column h in `out`
+            const int r = row_of(skip + h);
+            return ((int64_t)(cur.s.row + r) * hkv * group + cur.kh * group + skip + h - r * group) * d;
+        };
         auto store = [&](int h, int at, floatx4 x, float den) {
             if (at >= d) return;
             const float inv = den == 0.f ? 0.f : 1.f / den; // (a row that sees nothing: zeros)
             TX y[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) y[i] = (TX)(x[i] * inv);
-            __builtin_memcpy(out + ((int64_t)cur.s.row * hkv * group + h0 + h) * d + at, y, sizeof(y));
+            __builtin_memcpy(out + place_of(h) + at, y, sizeof(y));
         };
         for (int i = tid; i < heads * QUADS; i += THREADS) {
             const int h = i / QUADS, at = i % QUADS * 4;
@@ -464,12 +479,33 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
                 x += *(const floatx4 *)(ps_lds + (w * heads + h) * DP + at) * f;
                 den = fmaf(s_st[(w * 16 + h) * 2 + 1], f, den);
             }
+            if (max_new > 1 && !(0.f * x[0] + 0.f * x[1] + 0.f * x[2] + 0.f * x[3] + 0.f * den == 0.f)) s_bad[h] = 1;
             if (all) store(h, at, x, den);
             else {
 #pragma unroll
                 for (int e = 0; e < 4; e++) put(own + h * PITCH + at + e, x[e]);
                 if (at == 0) put(own + h * PITCH + DP, mx), put(own + h * PITCH + DP + 1, den);
             }
+        }
+        if (max_new > 1) { // (of one row: what it does not see was set to zeros)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // what was stored before
+            __syncthreads();
+            for (int h = wave; h < heads; h += NWV)
+                if (s_bad[h]) {
+                    const int r = row_of(skip + h), p = cur.s.p + r, from = (cur.s.first + cur.from) * TK, to = (cur.s.first + cur.to) * TK - 1;
+                    const int lo = window && p - window + 1 > from ? p - window + 1 : from, top = p < cur.s.end - 1 ? p : cur.s.end - 1;
+                    const PagedKv kv = {k_pages, v_pages, page_stride, head_stride, slot_stride, pages, shift};
+                    float m, l, o[4];
+                    paged_again<TX, TP>(q + (cur.s.row + r) * q_st + (cur.kh * group + skip + h - r * group) * q_sh, d, scale * 1.4426950408889634f, F16 ? 14.f : 0.f, kv,
+                                        table + (int64_t)cur.b * cols, cur.kh, lo, to < top ? to : top, m, l, o);
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    for (int e = 0; e < 4; e++)
+                        if (lane + 64 * e < d) {
+                            if (all) out[place_of(h) + lane + 64 * e] = (TX)(o[e] * inv);
+                            else put(own + h * PITCH + lane + 64 * e, o[e]);
+                        }
+                    if (!all && lane == 0) put(own + h * PITCH + DP, m), put(own + h * PITCH + DP + 1, l);
+                }
         }
         if (!all) {
             // the pair's workgroups (all stretches before the line's last are as long as this one, or this is the last)
@@ -485,7 +521,7 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
                 float *s_w = ps_lds, *s_l = ps_lds + parts * heads; // [head][part]: maxima, then weights; sums
                 // Groups of threads take parts in turn, the first EARLY of each along with the statistics.
                 const int items = heads * QUADS, groups = items < THREADS ? THREADS / items : 1, pg = groups > 1 ? tid / items : 0;
-                constexpr int EARLY = MIXED && !F16 ? 4 : 8;
+                constexpr int EARLY = MIXED ? 4 : 8;
                 floatx4 first[EARLY];
                 auto ask = [&](int i, int k) {
                     const float *p = part(k) + i / QUADS * PITCH + i % QUADS * 4;
@@ -541,23 +577,16 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
             }
         }
         __syncthreads(); // the next pair's results go to the same places
+        if (go && MIXED) ask_q(next);
         cur = next;
     }
 }
 
 template <typename TX, typename TP, int DP, int NWV>
-static fh_status ps_launch(fh_device *dev, const PagedCall &call, int max_len) {
-    constexpr int TK = sizeof(TP) == 4 ? 16 : 32;
-    const int group = call.hq / call.hkv, heads = group < 16 ? group : 16;
-    const int blocks = (group + 15) / 16, place = heads * (DP + 4);
-    int64_t longest = (int64_t)call.rows.cols << call.kv.shift;
-    if (max_len > 0 && max_len < longest) longest = max_len;
-    if (call.window > 0 && call.window + TK < longest) longest = call.window + TK;
-    const int64_t pairs = (int64_t)call.rows.seqs * call.hkv * blocks;
-    int whole = longest <= 4 * NWV * TK, least = NWV;
-    if (getenv("XW")) whole = atoi(getenv("XW"));
-    if (getenv("XL")) least = atoi(getenv("XL"));
-    unsigned grid = (unsigned)pairs;
+static fh_status ps_launch(fh_device *dev, const PagedCall &call, int whole) {
+    const int group = call.hq / call.hkv, wide = call.rows.max_new * group, heads = wide < 16 ? wide : 16;
+    const int blocks = (wide + 15) / 16, place = heads * (DP + 4);
+    unsigned grid = (unsigned)((int64_t)call.rows.seqs * call.hkv * blocks);
     if (!whole) {
         grid = (unsigned)dev->compute_units;
         FH_TRY(fh_dev_scratch(dev, (void **)&dev->part_buf, &dev->part_cap, (size_t)grid * 2 * place * 4));
@@ -570,15 +599,27 @@ static fh_status ps_launch(fh_device *dev, const PagedCall &call, int max_len) {
     FH_TRY(fh_kernel_lds(dev, (const void *)kern, lds));
     kern<<<dim3(grid), dim3(64 * NWV), lds, dev->stream>>>(call.rows.table, call.rows.lens, call.rows.starts, call.rows.cols, call.kv.shift, whole, call.hkv, blocks, call.window,
                                                            call.kv.pages, call.kv.k, call.kv.v, call.kv.page, call.kv.head, call.kv.slot, (const TX *)call.q, call.q_st, call.q_sh,
-                                                           group, call.d, call.scale, call.rows.seqs, call.rows.tokens, least, place, dev->part_buf, dev->arrived, (TX *)call.out);
+                                                           group, call.d, call.scale, call.rows.seqs, call.rows.tokens, call.rows.max_new, NWV, place, dev->part_buf, dev->arrived, (TX *)call.out);
     FH_HIP(hipGetLastError());
     return FH_OK;
 }
 template <typename TX, typename TP>
 static fh_status ps_dim(fh_device *dev, const PagedCall &call, int max_len) {
-    if (call.d <= 64) return ps_launch<TX, TP, 64, 8>(dev, call, max_len);
-    if (call.d <= 128) return ps_launch<TX, TP, 128, 8>(dev, call, max_len);
-    return ps_launch<TX, TP, 256, 4>(dev, call, max_len);
+    constexpr int TK = sizeof(TP) == 4 ? 16 : 32;
+    int64_t longest = (int64_t)call.rows.cols << call.kv.shift;
+    if (max_len > 0 && max_len < longest) longest = max_len;
+    const int64_t most = (int64_t)call.window + call.rows.max_new + TK;
+    if (call.window > 0 && most < longest) longest = most;
+    // A pair a workgroup of four wavefronts (two of them a compute unit), or the line's stretches of eight.  Few tiles are not worth the join; with a pair for every
+    // compute unit there is less to balance (32 / 8 heads of 128, f16, us, a pair / stretches: 1 sequence of 700 positions 11.3 / 17.5, 2000 22.8 / 16.6; 16 of 1500
+    // 20.7 / 24.0, 2000 28.5 / 25.8; 32 of 2048 38.1 / 41.7, 4096 70.8 / 70.1).  Pairs by eight wavefronts: 64 sequences of 100 12.7 / 8.5, 1 of 1000 14.6 / 13.6;
+    // stretches of four, two a compute unit: 1 of 131072 102 / 115.
+    const int wide = call.rows.max_new * (call.hq / call.hkv);
+    const int64_t tiles = (longest + TK - 1) / TK * (call.d > 128 ? 2 : 1), pairs = (int64_t)call.rows.seqs * call.hkv * ((wide + 15) / 16);
+    const bool whole = tiles <= 32 || (tiles <= 48 && 2 * pairs >= dev->compute_units) || (tiles <= 64 && pairs >= dev->compute_units);
+    if (call.d > 128) return ps_launch<TX, TP, 256, 4>(dev, call, whole);
+    if (call.d > 64) return whole ? ps_launch<TX, TP, 128, 4>(dev, call, true) : ps_launch<TX, TP, 128, 8>(dev, call, false);
+    return whole ? ps_launch<TX, TP, 64, 4>(dev, call, true) : ps_launch<TX, TP, 64, 8>(dev, call, false);
 }
 fh_status fh_paged_step(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len) {
     if (dtype == FH_F16) return ps_dim<fh_half, fh_half>(dev, call, max_len);

@@ -634,7 +634,9 @@ class PagedBatch:
         self.tokens = n if tokens is None else int(tokens)
         self.max_new = (1 if starts is None else self.tokens) if max_new is None else int(max_new)
         self.max_len = int(max_len)
-        self.args = (None if starts is None else starts.ptr, lens.ptr, table.ptr, cols, n, self.tokens)
+        # (as the calls take them: made once, not converted again in each)
+        self.args = (C.c_void_p(None if starts is None else starts.ptr), C.c_void_p(lens.ptr), C.c_void_p(table.ptr), C.c_int32(cols), C.c_int32(n),
+                     C.c_int32(self.tokens))
 
 
 class PagedKvCache:
@@ -660,8 +662,8 @@ class PagedKvCache:
         self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = shape
         row = self.page_size * self.head_dim
         step = k.nbytes // self.layers
-        self._layers = [(k.ptr + i * step, v.ptr + i * step, self.kv_heads * row, row, self.head_dim, self.pages, self.page_size)
-                        for i in range(self.layers)]
+        sizes = (C.c_int64(self.kv_heads * row), C.c_int64(row), C.c_int64(self.head_dim), C.c_int32(self.pages), C.c_int32(self.page_size))
+        self._layers = [(C.c_void_p(k.ptr + i * step), C.c_void_p(v.ptr + i * step), *sizes) for i in range(self.layers)]
 
     def layer(self, layer: int):
         """A layer's pointers, strides and sizes as the library takes them."""
