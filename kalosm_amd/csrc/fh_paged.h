@@ -101,7 +101,9 @@ struct PagedCall {
     float scale;
     int window, hq, hkv, d;
 };
-fh_status fh_paged_step(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len); // rows.max_new rows of all heads of a KV head: 16 at most, or one row
+// rows.max_new rows of a KV head's heads: one row, or up to 16 in all where fh_paged_step_whole.
+fh_status fh_paged_step(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len);
+bool fh_paged_step_whole(const fh_device *dev, int kv_dtype, const PagedCall &call, int max_len); // caches so short that a pair is one workgroup's
 fh_status fh_paged_prompt(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len);
 // The GPU of `dev` is the calling thread's current one while this lives.
 struct PagedGpu {

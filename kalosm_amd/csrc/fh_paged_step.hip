@@ -487,24 +487,19 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
                 if (at == 0) put(own + h * PITCH + DP, mx), put(own + h * PITCH + DP + 1, den);
             }
         }
-        if (max_new > 1) { // (of one row: what it does not see was set to zeros)
+        if (max_new > 1) { // several rows, and so a whole pair (of one row: what it does not see was set to zeros)
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // what was stored before
             __syncthreads();
             for (int h = wave; h < heads; h += NWV)
                 if (s_bad[h]) {
-                    const int r = row_of(skip + h), p = cur.s.p + r, from = (cur.s.first + cur.from) * TK, to = (cur.s.first + cur.to) * TK - 1;
-                    const int lo = window && p - window + 1 > from ? p - window + 1 : from, top = p < cur.s.end - 1 ? p : cur.s.end - 1;
+                    const int r = row_of(skip + h), p = cur.s.p + r;
                     const PagedKv kv = {k_pages, v_pages, page_stride, head_stride, slot_stride, pages, shift};
                     float m, l, o[4];
                     paged_again<TX, TP>(q + (cur.s.row + r) * q_st + (cur.kh * group + skip + h - r * group) * q_sh, d, scale * 1.4426950408889634f, F16 ? 14.f : 0.f, kv,
-                                        table + (int64_t)cur.b * cols, cur.kh, lo, to < top ? to : top, m, l, o);
+                                        table + (int64_t)cur.b * cols, cur.kh, window && p - window + 1 > 0 ? p - window + 1 : 0, p < cur.s.end - 1 ? p : cur.s.end - 1, m, l, o);
                     const float inv = l == 0.f ? 0.f : 1.f / l;
                     for (int e = 0; e < 4; e++)
-                        if (lane + 64 * e < d) {
-                            if (all) out[place_of(h) + lane + 64 * e] = (TX)(o[e] * inv);
-                            else put(own + h * PITCH + lane + 64 * e, o[e]);
-                        }
-                    if (!all && lane == 0) put(own + h * PITCH + DP, m), put(own + h * PITCH + DP + 1, l);
+                        if (lane + 64 * e < d) out[place_of(h) + lane + 64 * e] = (TX)(o[e] * inv);
                 }
         }
         if (!all) {
@@ -563,7 +558,7 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
 #pragma unroll
                         for (int k = 0; k < EARLY; k++)
                             if (pg + k * groups < parts) x += (base ? ask(i, pg + k * groups) : first[k]) * w[pg + k * groups];
-#pragma unroll 4
+#pragma unroll 8
                         for (int k = pg + EARLY * groups; k < parts; k += groups) x += ask(i, k) * w[k];
                     }
                     if (groups > 1) {
@@ -603,28 +598,30 @@ static fh_status ps_launch(fh_device *dev, const PagedCall &call, int whole) {
     FH_HIP(hipGetLastError());
     return FH_OK;
 }
-template <typename TX, typename TP>
-static fh_status ps_dim(fh_device *dev, const PagedCall &call, int max_len) {
-    constexpr int TK = sizeof(TP) == 4 ? 16 : 32;
+// A pair a workgroup of four wavefronts (two of them a compute unit), or the line's stretches of eight.  Few tiles are not worth the join; with a pair for every
+// compute unit there is less to balance (32 / 8 heads of 128, f16, us, a pair / stretches: 1 sequence of 700 positions 11.3 / 17.5, 2000 22.8 / 16.6; 16 of 1500
+// 20.7 / 24.0, 2000 28.5 / 25.8; 32 of 2048 38.1 / 41.7, 4096 70.8 / 70.1).  Pairs by eight wavefronts: 64 sequences of 100 12.7 / 8.5, 1 of 1000 14.6 / 13.6;
+// stretches of four, two a compute unit: 1 of 131072 102 / 115.
+bool fh_paged_step_whole(const fh_device *dev, int kv_dtype, const PagedCall &call, int max_len) {
+    const int TK = kv_dtype == FH_F32 ? 16 : 32, wide = call.rows.max_new * (call.hq / call.hkv);
     int64_t longest = (int64_t)call.rows.cols << call.kv.shift;
     if (max_len > 0 && max_len < longest) longest = max_len;
     const int64_t most = (int64_t)call.window + call.rows.max_new + TK;
     if (call.window > 0 && most < longest) longest = most;
-    // A pair a workgroup of four wavefronts (two of them a compute unit), or the line's stretches of eight.  Few tiles are not worth the join; with a pair for every
-    // compute unit there is less to balance (32 / 8 heads of 128, f16, us, a pair / stretches: 1 sequence of 700 positions 11.3 / 17.5, 2000 22.8 / 16.6; 16 of 1500
-    // 20.7 / 24.0, 2000 28.5 / 25.8; 32 of 2048 38.1 / 41.7, 4096 70.8 / 70.1).  Pairs by eight wavefronts: 64 sequences of 100 12.7 / 8.5, 1 of 1000 14.6 / 13.6;
-    // stretches of four, two a compute unit: 1 of 131072 102 / 115.
-    const int wide = call.rows.max_new * (call.hq / call.hkv);
     const int64_t tiles = (longest + TK - 1) / TK * (call.d > 128 ? 2 : 1), pairs = (int64_t)call.rows.seqs * call.hkv * ((wide + 15) / 16);
-    const bool whole = tiles <= 32 || (tiles <= 48 && 2 * pairs >= dev->compute_units) || (tiles <= 64 && pairs >= dev->compute_units);
+    return tiles <= 32 || (tiles <= 48 && 2 * pairs >= dev->compute_units) || (tiles <= 64 && pairs >= dev->compute_units);
+}
+template <typename TX, typename TP>
+static fh_status ps_dim(fh_device *dev, const PagedCall &call, bool whole) {
     if (call.d > 128) return ps_launch<TX, TP, 256, 4>(dev, call, whole);
     if (call.d > 64) return whole ? ps_launch<TX, TP, 128, 4>(dev, call, true) : ps_launch<TX, TP, 128, 8>(dev, call, false);
     return whole ? ps_launch<TX, TP, 64, 4>(dev, call, true) : ps_launch<TX, TP, 64, 8>(dev, call, false);
 }
 fh_status fh_paged_step(fh_device *dev, int dtype, int kv_dtype, const PagedCall &call, int max_len) {
-    if (dtype == FH_F16) return ps_dim<fh_half, fh_half>(dev, call, max_len);
-    if (dtype == FH_PAGED_BF16) return ps_dim<fh_bf, fh_bf>(dev, call, max_len);
-    if (kv_dtype == FH_F32) return ps_dim<float, float>(dev, call, max_len);
-    if (kv_dtype == FH_F16) return ps_dim<float, fh_half>(dev, call, max_len);
-    return ps_dim<float, fh_bf>(dev, call, max_len);
+    const bool whole = fh_paged_step_whole(dev, kv_dtype, call, max_len);
+    if (dtype == FH_F16) return ps_dim<fh_half, fh_half>(dev, call, whole);
+    if (dtype == FH_PAGED_BF16) return ps_dim<fh_bf, fh_bf>(dev, call, whole);
+    if (kv_dtype == FH_F32) return ps_dim<float, float>(dev, call, whole);
+    if (kv_dtype == FH_F16) return ps_dim<float, fh_half>(dev, call, whole);
+    return ps_dim<float, fh_bf>(dev, call, whole);
 }
