@@ -643,11 +643,14 @@ __global__ __launch_bounds__(256) void k_paged_join(PpArgs a) {
 }
 
 // ---------------------------------------------------------------- which form
-// Parts: as many as compute units have a workgroup each, with at least `least` positions; where scratch memory cannot be had, one.
-static int pp_parts(fh_device *dev, const PagedCall &call, int64_t wgs, int64_t longest, int least, PpArgs *a) {
-    int parts = (int)(dev->compute_units / wgs);
-    parts = (int)(longest / least < parts ? longest / least : parts);
+// Parts: as many as compute units have a workgroup each, of at least a step of positions; one where that saves a workgroup fewer than `saves` steps, which is what
+// the second launch takes (32 / 8 heads of 128, f16, us, with parts / without: 16 rows behind 500 positions 14.2 / 19.4, 8 behind 2000 16.3 / 39.6, a prompt of 300
+// 20.5 / 16.0, of 512 24.0 / 18.8; f32 10 behind 500 18.9 / 57), and where scratch memory cannot be had.
+static int pp_parts(fh_device *dev, const PagedCall &call, int64_t wgs, int64_t longest, int step, int saves, PpArgs *a) {
+    const int64_t steps = (longest + step - 1) / step;
+    int parts = (int)(dev->compute_units / wgs < steps ? dev->compute_units / wgs : steps);
     parts = parts < 1 ? 1 : parts > PP_PARTS ? PP_PARTS : parts;
+    if (steps - (steps + parts - 1) / parts < saves) parts = 1;
     a->parts = parts;
     if (parts == 1) return 1;
     const size_t n = (size_t)parts * call.rows.tokens * call.hq;
@@ -678,7 +681,7 @@ static fh_status pp_planes(fh_device *dev, PpArgs a, int64_t longest) {
     constexpr int KP = sizeof(TP) == 4 ? 3 : 1, LDS = KP * 32 * (DP + 8 + DP + 32) * 2;
     const int64_t blocks = ((int64_t)a.c.rows.max_new * (a.c.hq / a.c.hkv) + 127) / 128;
     a.sorted = blocks * a.c.hkv * a.c.rows.seqs > dev->compute_units;
-    pp_parts(dev, a.c, blocks * a.c.hkv * a.c.rows.seqs, longest, 256, &a);
+    pp_parts(dev, a.c, blocks * a.c.hkv * a.c.rows.seqs, longest, 64, 1, &a);
     const auto kern = k_paged_planes<TX, TP, DP>;
     FH_TRY(fh_kernel_lds(dev, (const void *)kern, LDS));
     kern<<<dim3((unsigned)a.c.hkv, (unsigned)blocks, (unsigned)(a.c.rows.seqs * a.parts)), dim3(256), LDS, dev->stream>>>(a);
@@ -696,7 +699,7 @@ template <typename T> static fh_status pp_same(fh_device *dev, PpArgs a, int64_t
     const int64_t wgs = pairs * ((rows + 127) / 128);
     const bool halves = wgs <= 2 * dev->compute_units && longest > 128;
     a.sorted = wgs > dev->compute_units;
-    pp_parts(dev, a.c, wgs, longest, 512, &a);
+    pp_parts(dev, a.c, wgs, longest, 128, 3, &a);
     if (a.c.d > 64) return halves ? pp_tiles<T, 128, 2>(dev, a) : pp_tiles<T, 128, 1>(dev, a);
     return halves ? pp_tiles<T, 64, 2>(dev, a) : pp_tiles<T, 64, 1>(dev, a);
 }
