@@ -3,7 +3,7 @@ and several (tiles of a prompt); slots that nothing may see hold NaN in every ca
 import numpy as np
 import pytest
 
-from pagedgen import Pages, near, unpack
+from pagedgen import Pages, near, pack, unpack
 from kalosm_amd.fusor import FusorHipError, PagedBatch, Tensor
 
 pytestmark = pytest.mark.gpu
@@ -128,7 +128,7 @@ def test_sharp_and_large_values(dev, new, act, kept):
 
 @pytest.mark.parametrize("act,kept", TYPES)
 def test_infinite_and_nan_rows_stay_theirs(dev, act, kept):
-    """An infinity or a NaN in V reaches the rows that see it, and no others; -inf in K takes its position out."""
+    """An infinity or a NaN in V reaches the rows that see it, and no others."""
     for new in ([1, 1, 1], [90, 1, 70]):
         p = Pages(31, new, [90, 200, 300], 4, 2, 64, 16, act, kept)
         inf = {"f32": np.float32(np.inf), "f16": np.float16(np.inf), "bf16": np.uint16(0x7F80)}[kept]
@@ -232,3 +232,109 @@ def test_refused(dev):
         Tensor.zeros(dev, (1, 3, 64), "f16").paged_attention(cache, batch, 0.1)
     with pytest.raises(FusorHipError, match="layer 1"):
         Tensor.zeros(dev, (1, 4, 64), "f16").paged_attention(cache, batch, 0.1, layer=1)
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+@pytest.mark.parametrize("hq,hkv,new", [(8, 2, [4, 1, 3, 0, 4]), (2, 2, [16, 2, 7, 16, 1]), (5, 1, [3, 3, 1, 2, 3]), (8, 1, [2, 2, 0, 1, 2])])
+@pytest.mark.parametrize("d", [64, 128, 200])
+def test_few_rows(dev, act, kept, hq, hkv, new, d):
+    """Up to 16 rows of a KV head's heads behind short caches: columns of one tile, each with a limit of its own."""
+    lens = [90, 1, 17, 33, 300]
+    lens = [max(a, b) for a, b in zip(lens, new)]
+    p = Pages(hq + d, new, lens, hq, hkv, d, 16, act, kept)
+    check(dev, p, what=f"{new} rows of {hq}/{hkv} heads of {d}")
+    check(dev, p, 9, what=f"{new} rows of {hq}/{hkv} heads of {d}, a window of 9")
+    p.table[0, 2], p.table[4, 0], p.table[4, 7] = -1, p.pages, -3
+    check(dev, p, what=f"{new} rows, holes")
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+def test_infinities_and_nan_of_few_rows(dev, act, kept):
+    """A row does not see what its neighbour behind it sees, whatever that is."""
+    for new in ([3, 1, 2], [4, 4, 4]):
+        p = Pages(33, new, [90, 40, 300], 4, 2, 64, 16, act, kept)
+        for i, bits in ((0, np.nan), (2, np.inf), (1, -np.inf)):
+            pos = p.lens[i] - 1
+            p.v[p.table[i, pos // 16], :, pos % 16, 5 + i] = pack(np.full(2, bits), kept)
+        got = run(dev, p)
+        with np.errstate(invalid="ignore"):
+            want, bound = p.attention(64 ** -0.5)
+        fine = np.isfinite(want)
+        assert (~fine).sum() == 3 * 4 and (np.isfinite(got) == fine).all(), f"{new}: {np.argwhere(np.isfinite(got) != fine)[:5].tolist()}"
+        near(np.where(fine, got, 0), np.where(fine, want, 0), np.where(fine, bound, 1), f"{act}/{kept} {new}")
+
+
+@pytest.mark.parametrize("act,kept", [("f16", "f16"), ("f32", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (18, 1)])
+def test_a_hundred_ragged_sequences(dev, act, kept, hq, hkv):
+    """More sequences than a wavefront has lanes, long and empty ones among them: the line's stretches begin anywhere."""
+    rng = np.random.default_rng(7)
+    lens = [int(x) for x in rng.integers(0, 200, 150)]
+    lens[3], lens[70], lens[71], lens[140] = 3000, 2500, 0, 4111
+    new = [1] * 150
+    new[5], new[64], new[149] = 0, 0, 0
+    p = Pages(14, new, lens, hq, hkv, 64, 32, act, kept)
+    check(dev, p, what="150 sequences")
+    check(dev, p, 2100, what="150 sequences, a window")
+    p.table[3, 20:40], p.table[140, 0], p.table[140, 128] = -1, -1, -1
+    check(dev, p, what="150 sequences, holes")
+
+
+def test_more_sequences_than_sorted(dev):
+    """Prompts of more workgroups than run at once: the longest first, of up to 64 sequences, and as they come of more."""
+    rng = np.random.default_rng(8)
+    for n in (40, 64, 65):
+        new = [int(x) for x in rng.integers(0, 90, n)]
+        lens = [a + int(b) for a, b in zip(new, rng.integers(0, 200, n))]
+        lens[1:4] = [lens[0]] * 3  # equals
+        new[1:4] = [min(x, lens[0]) for x in new[1:4]]
+        p = Pages(n, new, lens, 16, 8, 64, 16, "bf16", "bf16")
+        check(dev, p, what=f"{n} prompts")
+
+
+def test_a_pool_of_more_than_four_gigabytes(dev):
+    """Pages whose bytes lie past 2^32, written and read."""
+    pages, page, d = 2200, 1024, 128
+    pool = Tensor(dev, (pages, 8, page, d), "f16")  # 4.6 GB, K and V alike
+    from kalosm_amd.fusor import PagedKvCache
+    cache = PagedKvCache.over(pool, pool)
+    rng = np.random.default_rng(9)
+    for new in ([1, 1], [40, 1100]):
+        table = np.array([[2199, 0], [2150, 2197]], np.int32)
+        n = sum(new)
+        starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        batch = PagedBatch(Tensor.from_slice(dev, np.array(new, np.int32), "i32"), Tensor.from_slice(dev, table, "i32"), Tensor.from_slice(dev, starts, "i32"),
+                           tokens=n, max_new=max(new), max_len=max(new))
+        k = pack(rng.standard_normal((n, 8, d)), "f16")
+        q = pack(rng.standard_normal((n, 8, d)), "f16")
+        kt = Tensor.from_slice(dev, k, "f16")
+        cache.append(kt, kt, batch)
+        got = unpack(Tensor.from_slice(dev, q, "f16").paged_attention(cache, batch, d ** -0.5).as_slice(), "f16")
+        for i, m in enumerate(new):
+            x, y = unpack(q[starts[i]:starts[i + 1]], "f16"), unpack(k[starts[i]:starts[i + 1]], "f16")
+            s = np.einsum("ahd,bhd->hab", x, y) * d ** -0.5
+            s[:, np.triu(np.ones((m, m), bool), 1)] = -np.inf
+            w = np.exp(s - s.max(-1, keepdims=True))
+            w /= w.sum(-1, keepdims=True)
+            want = np.einsum("hab,bhd->ahd", w, y)
+            # weights and results rounded to f16: half a step each of at most sum w |v|
+            assert np.abs(got[starts[i]:starts[i + 1]] - want).max() <= 2.1 * 2.0 ** -11 * np.abs(y).max(), (new, i)
+
+
+def test_without_scratch_memory(dev):
+    """Prompts that cannot have memory for their parts run in one; a captured call as well."""
+    p = Pages(17, [20], [3000], 4, 1, 128, 16, "bf16", "bf16")
+    from kalosm_amd.fusor import Device
+    alone = Device.gpu(0)
+    alone.set_option("scratch_limit", 1)
+    cache, batch = p.put(alone)
+    q, out = Tensor.from_slice(alone, p.q, p.act), Tensor.zeros(alone, p.q.shape, p.act)
+    want, bound = p.attention(128 ** -0.5)
+    q.paged_attention(cache, batch, 128 ** -0.5, out=out)
+    near(unpack(out.as_slice(), p.act), want, bound, "no scratch memory")
+    alone.graph_begin()
+    q.paged_attention(cache, batch, 128 ** -0.5, out=out)
+    g = alone.graph_end()
+    for _ in range(3):
+        g.launch()
+        near(unpack(out.as_slice(), p.act), want, bound, "no scratch memory, captured")
