@@ -321,7 +321,10 @@ fh_status fh_flash_attention_decode_static(fh_device *dev, int32_t q_dtype, int3
  *            nor those behind the table's last column.  So a sequence that only looks back a window may give pages back.
  * dtype is the type of q, k, v and out, kv_dtype that of the pages: FH_F32, FH_F16 or FH_DECODER_BF16, both alike or f32
  * rows over 16-bit pages.  head_dim is a multiple of 8 up to 256.  All sums and softmax statistics are f32.
- * Lengths, starts and tables are read on the device when the call runs: a captured graph takes what they hold at replay. */
+ * Lengths, starts and tables are read on the device when the call runs: a captured graph takes what they hold at replay.
+ * Infinities and NaN among the keys and values that a row sees may make its results infinities or NaN; what it does not
+ * see (later rows, positions before its window, slots that no position has reached) makes no difference, whatever it is.
+ * At most 65535 heads and sequences, and 2^29 positions of a sequence, rows and pages. */
 
 /* q and k turned by their positions (RopeCache::forward{,_interleaved}, fusor-ml/fusor/src/composite/rope.rs:284-329; with
  * several axes as models/kalosm-llama/src/raw/rope.rs does for pictures), k and v written to their pages.  q is
@@ -346,9 +349,12 @@ fh_status fh_paged_rope_append(fh_device *dev, int32_t dtype, int32_t kv_dtype, 
  * window > 0 only those with j > p - window.  q is [tokens, hq, d] with strides q_st and q_sh (elements), out contiguous
  * [tokens, hq, d]; query head h reads KV head h / (hq / hkv).  A row that sees nothing gets zeros.  scale: 2^-60 and above.
  * max_new: the most rows a sequence has; of sequences with more, the first max_new are computed and the rest left as they
- * were.  With 1 (a decode step) every cache is split over the device and joined in the same launch; with more the rows run on
- * the tiles of a prompt.  max_len: the longest sequence, or 0 where the host does not know; it chooses between forms of the
- * kernels and nothing else.  Results do not depend on which pages hold a sequence. */
+ * were.  With 1 (a decode step) long caches are split over the device and joined in the same launch; with more the rows run on
+ * the tiles of a prompt, split over a long cache where they are few, and joined by a second launch.  max_new * hq / hkv is at
+ * most 4194240.  max_len: the longest sequence, or 0 where the host does not know; it chooses between forms of the
+ * kernels, whose results differ by their rounding, and nothing else.  Results do not depend on which pages hold a sequence, and
+ * are the same bits in every run.  Parts of a split cache meet in scratch memory that the device handle grows: captured calls
+ * need an eager one of their size before (prompts that find none run unsplit). */
 fh_status fh_paged_attention(fh_device *dev, int32_t dtype, int32_t kv_dtype, const void *q_dev, int64_t q_st, int64_t q_sh,
                              int32_t hq, int32_t hkv, int32_t d, float scale, int32_t window, const void *k_pages_dev,
                              const void *v_pages_dev, int64_t page_stride, int64_t head_stride, int64_t slot_stride,

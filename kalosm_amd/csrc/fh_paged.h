@@ -62,8 +62,14 @@ __device__ __forceinline__ void paged_again(const TX *q, int d, float sc2, float
             if ((unsigned)page < (unsigned)kv.pages) {
                 at = page * kv.page + kh * kv.head + (key & ((1 << kv.shift) - 1)) * kv.slot;
                 y = 0.f;
-#pragma unroll 1
-                for (int e = 0; e < d; e++) y = fmaf((float)q[e], (float)((const TP *)(kv.k + at))[e], y);
+#pragma unroll 1 // (few registers: it stands behind loops that have none left)
+                for (int e = 0; e < d; e += 8) { // (multiples of 8 at multiples of 16 bytes)
+                    TP x[8];
+                    uint4 w[sizeof(TP) / 2];
+                    for (int i = 0; i < (int)sizeof(TP) / 2; i++) w[i] = ((const uint4 *)(kv.k + at + e * (int)sizeof(TP)))[i];
+                    __builtin_memcpy(x, w, sizeof(x));
+                    for (int i = 0; i < 8; i++) y = fmaf((float)q[e + i], (float)x[i], y);
+                }
                 y *= sc2;
             }
         }
@@ -76,7 +82,7 @@ __device__ __forceinline__ void paged_again(const TX *q, int d, float sc2, float
         for (int w = 32; w; w >>= 1) sum += __shfl_xor(sum, w);
         l = l * alpha + sum;
         for (int e = 0; e < 4; e++) o[e] *= alpha;
-#pragma unroll 1 // (few registers: it stands behind loops that have none left)
+#pragma unroll 4
         for (int j = 0; j < 64; j++) {
             const int64_t v = __shfl(at, j);
             const float p = __shfl(pr, j);
@@ -84,6 +90,9 @@ __device__ __forceinline__ void paged_again(const TX *q, int d, float sc2, float
                 for (int e = 0; e < 4; e++)
                     if (lane + 64 * e < d) o[e] = fmaf(p, (float)((const TP *)(kv.v + v))[lane + 64 * e], o[e]);
         }
+        bool lost = true; // nothing that comes makes any of it finite again
+        for (int e = 0; e < 4; e++) lost &= lane + 64 * e >= d || !(0.f * o[e] == 0.f);
+        if (__all(lost || !(0.f * l == 0.f))) return;
     }
 }
 

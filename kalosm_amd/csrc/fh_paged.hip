@@ -31,7 +31,7 @@ fh_status fh_paged_arguments(int dtype, int kv_dtype, int hq, int hkv, int d, co
     if (d % 8 || d > 256) FH_FAIL(FH_ERR_UNSUPPORTED, "head_dim %d: paged attention takes multiples of 8 up to 256", d);
     if (page_size < 16 || page_size > 4096 || (page_size & (page_size - 1)))
         FH_FAIL(FH_ERR_UNSUPPORTED, "pages of %d positions: powers of two from 16 to 4096 are supported", page_size);
-    FH_REQUIRE(hq <= 65535 && seqs <= 65535 && pages <= FH_PAGED_MAX, "at most 65535 heads and sequences and 2^29 pages");
+    FH_REQUIRE(hq <= 65535 && seqs <= 65535 && pages <= FH_PAGED_MAX && tokens <= FH_PAGED_MAX, "at most 65535 heads and sequences and 2^29 pages and rows");
     FH_REQUIRE((int64_t)cols * page_size <= FH_PAGED_MAX, "a table row of %d pages of %d positions reaches past 2^29", cols, page_size);
     FH_REQUIRE(starts || tokens == seqs, "%d rows of %d sequences need their starts", tokens, seqs);
     const int size = kv_dtype == FH_F32 ? 4 : 2;
@@ -319,7 +319,7 @@ extern "C" fh_status fh_paged_attention(fh_device *dev, int32_t dtype, int32_t k
     rows.max_new = max_new < tokens ? max_new : tokens;
     PagedGpu gpu;
     FH_TRY(gpu.enter(dev));
-    const PagedCall call = {q_dev, out_dev, q_st, q_sh, kv, rows, scale, window, hq, hkv, d};
+    const PagedCall call = {q_dev, out_dev, q_st, q_sh, kv, rows, scale, window < FH_PAGED_MAX ? window : FH_PAGED_MAX, hq, hkv, d};
     // A few rows behind a short cache: as single tokens, the rows' heads as columns (32 / 8 heads of 128, f16, us, 2 rows behind 300 positions 8.5, by the tiles of a
     // prompt 14.1; 4 behind 1000 of 8 sequences 16.3 / 25.3).  Longer caches are cut into parts for either, and the tiles' are joined sooner (4 rows
     // behind 2000 25.1 / 23.1, 65536 73.8 / 60.2).

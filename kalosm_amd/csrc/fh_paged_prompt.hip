@@ -9,9 +9,9 @@
 // grid (KV heads, blocks of rows - the last, longest ones first -, sequences x parts).  With fewer workgroups than compute units the
 // positions are split over `parts` workgroups, whose sums go to scratch memory in f32 and are added up by a second launch.
 //
-// Positions that a row does not see have weight 0, whatever lies there: scores are replaced, and where a row's sums end up infinite or NaN -
-// 0 times an infinity or a NaN among the values of its last tile, say, or terms of an infinite f32 - the row is worked out again in f32 over
-// what it sees (pp_again): one at a time by a wavefront, slow, and never entered by finite caches.
+// Positions that a row does not see have weight 0, whatever lies there: scores are replaced, and where a row's sums end up infinite or NaN and a position in its
+// tiles that some row does not see has an infinity or a NaN - 0 times that is NaN - the row is worked out again in f32 over what it sees (pp_mend): one at a
+// time by a wavefront, until nothing of it can be finite.  (Looked for in the tiles as they come, by the sums before and behind them, 8192 tokens take 660 us for 626.)
 #include "fh_attention_tiles.h"
 #include "fh_paged.h"
 #include <type_traits>
@@ -111,10 +111,11 @@ __device__ __forceinline__ void pp_again(const PpArgs &a, int part, int seq, con
         }
     if (a.parts > 1 && lane == 0) a.stats[2 * where] = m, a.stats[2 * where + 1] = l;
 }
-// The rows of a wavefront (from first on, `rows` of the sequence in all) whose sums are not finite, again.
+// The rows of a wavefront, first .. first + 31 of the sequence's `rows`, whose sums are not finite, again, where positions from .. to have an infinity or a NaN
+// among the values that not all of them see.
 template <typename TX, typename TP, int D>
-__device__ __forceinline__ void pp_check(const PpArgs &a, int part, int seq, const PagedSeq &s, int first, int rows, int kh, int group, int from, int to, float l,
-                                         const floatx16 (&acc)[D / 32]) {
+__device__ __forceinline__ void pp_mend(const PpArgs &a, int part, int seq, const PagedSeq &s, const PpRow &x, int first, int rows, int kh, int group, int from, int to, bool holed,
+                                        float l, const floatx16 (&acc)[D / 32]) {
     float sum = 0.f * l; // (of 0 times everything)
 #pragma unroll
     for (int dt = 0; dt < D / 32; dt++)
@@ -123,6 +124,28 @@ __device__ __forceinline__ void pp_check(const PpArgs &a, int part, int seq, con
     uint64_t bad = __ballot(!(sum == 0.f));
     bad = (bad | bad >> 32) & 0xFFFFFFFFu;
     if (!bad) return;
+    // what lies behind the first row's end, and in front of the last one's beginning
+    const PagedKv &kv = a.c.kv;
+    const int lane = threadIdx.x & 63, pieces = a.c.d * (int)sizeof(TP) / 16;
+    int high = x.high, low = x.low;
+    for (int w = 32; w; w >>= 1) {
+        const int h = __shfl_xor(high, w), y = __shfl_xor(low, w);
+        high = h < high ? h : high, low = y > low ? y : low;
+    }
+    to = to < s.len - 1 ? to : s.len - 1;
+    const int begin = high + 1 > from ? high + 1 : from, behind = to >= begin ? to - begin + 1 : 0, ahead = low <= to ? (low > from ? low - from : 0) : to - from + 1;
+    bool wild = holed; // (what was read for a hole may be anything)
+    for (int i = lane; i < (behind + ahead) * pieces; i += 64) {
+        const int n = i / pieces, p = n < behind ? begin + n : from + n - behind, page = a.c.rows.table[(int64_t)seq * a.c.rows.cols + (p >> kv.shift)];
+        if ((unsigned)page >= (unsigned)kv.pages) wild = true;
+        else {
+            const uint4 w = *(const uint4 *)(kv.v + page * kv.page + kh * kv.head + (p & ((1 << kv.shift) - 1)) * kv.slot + (i - n * pieces) * 16);
+            TP v[16 / sizeof(TP)];
+            __builtin_memcpy(v, &w, 16);
+            for (int e = 0; e < 16 / (int)sizeof(TP); e++) wild |= !(0.f * (float)v[e] == 0.f);
+        }
+    }
+    if (!__any(wild)) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // what was stored before
     for (int i = 0; i < 32; i++)
         if (bad >> i & 1 && first + i < rows) pp_again<TX, TP>(a, part, seq, s, first + i, kh, group, from, to);
@@ -260,10 +283,10 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(2, 2))
         uint32_t holes = 0; // its 16s without a page
         if (holed)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int p = t0 + 16 * i;
-            if ((unsigned)column(p < last16 ? p : last16) >= (unsigned)kv.pages) holes |= 1u << i;
-        }
+            for (int i = 0; i < 4; i++) {
+                const int p = t0 + 16 * i;
+                if ((unsigned)column(p < last16 ? p : last16) >= (unsigned)kv.pages) holes |= 1u << i;
+            }
         if (__any(t0 + BN - 1 > x.high || t0 < x.low) || holes) // some row does not see the whole tile
 #pragma unroll
             for (int kt = 0; kt < 2; kt++)
@@ -386,7 +409,7 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(2, 2))
     if (KS == 2 && kset == 1) return;
     l_run = ap_swap32_sum(l_run);
     if (r < s.rows * group) pp_store<T, D>(a, part, s, x, kh, group, g, m_run, l_run, acc);
-    pp_check<T, T, D>(a, part, seq, s, r0 + (wave % QW) * 32, s.rows * group, kh, group, span.base, span.base + steps * KS * BN - 1, l_run, acc);
+    pp_mend<T, T, D>(a, part, seq, s, x, r0 + (wave % QW) * 32, s.rows * group, kh, group, span.base, span.base + steps * KS * BN - 1, holed, l_run, acc);
 }
 
 // ---------------------------------------------------------------- every other type and head_dim
@@ -461,6 +484,7 @@ __global__ __launch_bounds__(256) void k_paged_planes(PpArgs a) {
     const int last16 = (s.len - 1) & ~15;
     uint4 kraw[N][KP == 3 ? 2 : 1], vraw[N][KP == 3 ? 2 : 1];
     uint32_t holes = 0, next_holes = 0;
+    bool holed = false;
     int page[2];
     auto look = [&](int t0) {
 #pragma unroll
@@ -525,7 +549,7 @@ __global__ __launch_bounds__(256) void k_paged_planes(PpArgs a) {
             keep(kraw[i], sk + y * KR + e, BN * KR);
             keep(vraw[i], sv + y * VR + e, BN * VR);
         }
-        holes = next_holes;
+        holes = next_holes, holed |= holes != 0;
         __syncthreads();
         if (it + 1 < span.steps) {
             ask(t0 + BN);
@@ -594,7 +618,7 @@ __global__ __launch_bounds__(256) void k_paged_planes(PpArgs a) {
     }
     l_run = ap_swap32_sum(l_run);
     if (r < s.rows * group) pp_store<TX, DP>(a, part, s, x, kh, group, g, m_run, l_run, acc);
-    pp_check<TX, TP, DP>(a, part, seq, s, r0 + wave * 32, s.rows * group, kh, group, span.base, span.base + span.steps * BN - 1, l_run, acc);
+    pp_mend<TX, TP, DP>(a, part, seq, s, x, r0 + wave * 32, s.rows * group, kh, group, span.base, span.base + span.steps * BN - 1, holed, l_run, acc);
 }
 
 // ---------------------------------------------------------------- the parts together

@@ -338,3 +338,25 @@ def test_without_scratch_memory(dev):
     for _ in range(3):
         g.launch()
         near(unpack(out.as_slice(), p.act), want, bound, "no scratch memory, captured")
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+@pytest.mark.parametrize("new,lens", [([100, 40], [400, 40]), ([4, 2], [400, 9]), ([70], [3000])])
+@pytest.mark.parametrize("window", [0, 80])
+def test_nan_rows_anywhere(dev, act, kept, new, lens, window):
+    """Positions that hold nothing but NaN: in front of every row, between the rows, behind a window's beginning, everywhere."""
+    p = Pages(35, new, lens, 4, 2, 64, 16, act, kept)
+    nan = pack(np.array(np.nan), kept)
+
+    def spoil(i, pos):
+        for a in (p.k, p.v):
+            a[p.table[i, pos // 16], :, pos % 16] = nan
+
+    for places in ([(0, lens[0] - 2)], [(0, lens[0] - 30)], [(0, lens[0] - 90)], [(0, 5)], [(i, q) for i in range(len(lens)) for q in range(lens[i])]):
+        for i, pos in places:
+            spoil(i, pos)
+        got = run(dev, p, window)
+        want, bound = p.attention(64 ** -0.5, window)
+        fine = np.isfinite(want)
+        assert (np.isfinite(got) == fine).all(), f"{places[:1]}: {np.argwhere(np.isfinite(got) != fine)[:5].tolist()}"
+        near(np.where(fine, got, 0), np.where(fine, want, 0), np.where(fine, bound, 1), f"{act}/{kept} {new} {places[:1]}")
