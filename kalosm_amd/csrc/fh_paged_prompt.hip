@@ -112,10 +112,11 @@ __device__ __forceinline__ void pp_again(const PpArgs &a, int part, int seq, con
     if (a.parts > 1 && lane == 0) a.stats[2 * where] = m, a.stats[2 * where + 1] = l;
 }
 // The rows of a wavefront, first .. first + 31 of the sequence's `rows`, whose sums are not finite, again, where positions from .. to have an infinity or a NaN
-// among the values that not all of them see.
+// among the values that not all of them see.  And rows whose scores' largest, m, is of 2^25 or more, next to f16: what 14 - m is rounded by, and m itself, takes
+// weights out of f16's range.
 template <typename TX, typename TP, int D>
 __device__ __forceinline__ void pp_mend(const PpArgs &a, int part, int seq, const PagedSeq &s, const PpRow &x, int first, int rows, int kh, int group, int from, int to, bool holed,
-                                        float l, const floatx16 (&acc)[D / 32]) {
+                                        float m, float l, const floatx16 (&acc)[D / 32]) {
     float sum = 0.f * l; // (of 0 times everything)
 #pragma unroll
     for (int dt = 0; dt < D / 32; dt++)
@@ -123,7 +124,9 @@ __device__ __forceinline__ void pp_mend(const PpArgs &a, int part, int seq, cons
         for (int r = 0; r < 16; r++) sum = fmaf(0.f, acc[dt][r], sum);
     uint64_t bad = __ballot(!(sum == 0.f));
     bad = (bad | bad >> 32) & 0xFFFFFFFFu;
-    if (!bad) return;
+    uint64_t rounded = __ballot(__is_same(TP, fh_half) && fabsf(m) >= 0x1p25f && fabsf(m) < INFINITY);
+    rounded = (rounded | rounded >> 32) & 0xFFFFFFFFu;
+    if (!(bad | rounded)) return;
     // what lies behind the first row's end, and in front of the last one's beginning
     const PagedKv &kv = a.c.kv;
     const int lane = threadIdx.x & 63, pieces = a.c.d * (int)sizeof(TP) / 16;
@@ -145,7 +148,8 @@ __device__ __forceinline__ void pp_mend(const PpArgs &a, int part, int seq, cons
             for (int e = 0; e < 16 / (int)sizeof(TP); e++) wild |= !(0.f * (float)v[e] == 0.f);
         }
     }
-    if (!__any(wild)) return;
+    bad = __any(wild) ? bad | rounded : rounded;
+    if (!bad) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // what was stored before
     for (int i = 0; i < 32; i++)
         if (bad >> i & 1 && first + i < rows) pp_again<TX, TP>(a, part, seq, s, first + i, kh, group, from, to);
@@ -409,7 +413,7 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(2, 2))
     if (KS == 2 && kset == 1) return;
     l_run = ap_swap32_sum(l_run);
     if (r < s.rows * group) pp_store<T, D>(a, part, s, x, kh, group, g, m_run, l_run, acc);
-    pp_mend<T, T, D>(a, part, seq, s, x, r0 + (wave % QW) * 32, s.rows * group, kh, group, span.base, span.base + steps * KS * BN - 1, holed, l_run, acc);
+    pp_mend<T, T, D>(a, part, seq, s, x, r0 + (wave % QW) * 32, s.rows * group, kh, group, span.base, span.base + steps * KS * BN - 1, holed, m_run, l_run, acc);
 }
 
 // ---------------------------------------------------------------- every other type and head_dim
@@ -618,7 +622,7 @@ __global__ __launch_bounds__(256) void k_paged_planes(PpArgs a) {
     }
     l_run = ap_swap32_sum(l_run);
     if (r < s.rows * group) pp_store<TX, DP>(a, part, s, x, kh, group, g, m_run, l_run, acc);
-    pp_mend<TX, TP, DP>(a, part, seq, s, x, r0 + wave * 32, s.rows * group, kh, group, span.base, span.base + span.steps * BN - 1, holed, l_run, acc);
+    pp_mend<TX, TP, DP>(a, part, seq, s, x, r0 + wave * 32, s.rows * group, kh, group, span.base, span.base + span.steps * BN - 1, holed, m_run, l_run, acc);
 }
 
 // ---------------------------------------------------------------- the parts together

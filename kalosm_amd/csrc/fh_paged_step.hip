@@ -383,8 +383,17 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
 #pragma unroll
             for (int h = 0; h < HALVES; h++)
 #pragma unroll
+                for (int i = 0; i < 4; i++) p[h][i] = fmaf(st[h][i], sc2, sub);
+            if (F16 && __any(fabsf(ref) >= 0x1p25f)) // what 14 - ref is rounded by, and ref itself, would take weights out of f16's range
+#pragma unroll
+                for (int h = 0; h < HALVES; h++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) p[h][i] = st[h][i] * sc2 - ref + 14.f;
+#pragma unroll
+            for (int h = 0; h < HALVES; h++)
+#pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    p[h][i] = __builtin_amdgcn_exp2f(fmaf(st[h][i], sc2, sub));
+                    p[h][i] = __builtin_amdgcn_exp2f(p[h][i]);
                     ps += p[h][i];
                 }
             l_run = l_run * alpha + ps; // of this lane's keys: the four rows of a column are added at the end

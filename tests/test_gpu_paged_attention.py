@@ -360,3 +360,31 @@ def test_nan_rows_anywhere(dev, act, kept, new, lens, window):
         fine = np.isfinite(want)
         assert (np.isfinite(got) == fine).all(), f"{places[:1]}: {np.argwhere(np.isfinite(got) != fine)[:5].tolist()}"
         near(np.where(fine, got, 0), np.where(fine, want, 0), np.where(fine, bound, 1), f"{act}/{kept} {new} {places[:1]}")
+
+
+@pytest.mark.parametrize("act", ["f16", "f32"])
+@pytest.mark.parametrize("d", [64, 200])
+@pytest.mark.parametrize("new,lens", [([1] * 24, [100] * 24), ([1, 1], [9000, 3000]), ([4] * 9, [60] * 9), ([300, 100], [300, 900])])
+def test_scores_past_the_steps_of_their_sums(dev, act, d, new, lens):
+    """Scores of 2^23 to 2^29, where the largest, and 14 - the largest, are rounded by up to 32: the one that is largest has all of the weight.
+
+    Its weight in f16, and the result, are each off by half a step at most: together 2 * 2^-11 of the value, and terms of second order and of f32."""
+    p = Pages(91, new, lens, 4, 2, d, 16, act, "f16")
+    rng = np.random.default_rng(92)
+    values = np.arange(0x7100, 0x7C00, dtype=np.uint16).view(np.float16)  # 10240 and more, all different
+    p.k[:], p.q[:] = 0, 0
+    p.k[:, :, :, 0] = 1
+    tops = []
+    for i, n in enumerate(lens):
+        pos = np.arange(n)
+        at = rng.permutation(n)[:len(values)]  # the others stay at 1
+        p.k[p.table[i, at // 16], :, at % 16, 0] = rng.permutation(values)[:len(at), None]
+        tops.append(np.maximum.accumulate(p.k[p.table[i, pos // 16], 0, pos % 16, 0].astype(np.float64)))
+    p.q[:, :, 0] = pack(unpack(pack(rng.uniform(4000, 60000, (p.tokens, 4)), "f16"), "f16"), act)
+    got = run(dev, p)
+    want = np.zeros_like(got)
+    for row, i, last in p.rows():
+        j = np.arange(last + 1)
+        top = int(j[p.k[p.table[i, j // 16], 0, j % 16, 0].astype(np.float64) == tops[i][last]][0])
+        want[row] = np.repeat(unpack(p.v[p.table[i, top // 16], :, top % 16], "f16"), 2, 0)
+    near(got, want, 2.01 * 2.0 ** -11 * np.abs(want) + 2.0 ** -24, f"{act} {d} {new[:3]}")
