@@ -324,6 +324,8 @@ fh_status fh_flash_attention_decode_static(fh_device *dev, int32_t q_dtype, int3
  * Lengths, starts and tables are read on the device when the call runs: a captured graph takes what they hold at replay.
  * Infinities and NaN among the keys and values that a row sees may make its results infinities or NaN; what it does not
  * see (later rows, positions before its window, slots that no position has reached) makes no difference, whatever it is.
+ * Results are f32 sums of the values, each times a weight of up to 2^8 (next to f16: 2^16), over the sum of the weights:
+ * where f32 or bf16 values are so large that these sums pass 2^128, the results are infinities.
  * At most 65535 heads and sequences, and 2^29 positions of a sequence, rows and pages. */
 
 /* q and k turned by their positions (RopeCache::forward{,_interleaved}, fusor-ml/fusor/src/composite/rope.rs:284-329; with

@@ -388,3 +388,19 @@ def test_scores_past_the_steps_of_their_sums(dev, act, d, new, lens):
         top = int(j[p.k[p.table[i, j // 16], 0, j % 16, 0].astype(np.float64) == tops[i][last]][0])
         want[row] = np.repeat(unpack(p.v[p.table[i, top // 16], :, top % 16], "f16"), 2, 0)
     near(got, want, 2.01 * 2.0 ** -11 * np.abs(want) + 2.0 ** -24, f"{act} {d} {new[:3]}")
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 200])
+@pytest.mark.parametrize("new,lens", [([150, 40], [150, 700]), ([40], [4000]), ([3, 1], [200, 300])])
+@pytest.mark.parametrize("rise", [0.02, 0.11, -0.11, 1.0])
+def test_scores_that_rise(dev, act, kept, d, new, lens, rise):
+    """Scores that grow a little or much from a tile of positions to the next, and such that fall."""
+    p = Pages(93, new, lens, 4, 2, d, 16, act, kept)
+    for i, n in enumerate(lens):
+        pos = np.arange(n)
+        p.k[p.table[i, pos // 16], :, pos % 16, 0] = pack(rise * (pos - n)[:, None] * np.ones(2), kept)
+    q = unpack(p.q, act)
+    q[:, :, 0] = d ** 0.5 * np.array([1, 0.5, 1, 2])
+    p.q = pack(q, act)
+    check(dev, p, what=f"{rise} a position")
