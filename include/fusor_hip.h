@@ -326,6 +326,8 @@ fh_status fh_flash_attention_decode_static(fh_device *dev, int32_t q_dtype, int3
  * see (later rows, positions before its window, slots that no position has reached) makes no difference, whatever it is.
  * Results are f32 sums of the values, each times a weight of up to 2^8 (next to f16: 2^16), over the sum of the weights:
  * where f32 or bf16 values are so large that these sums pass 2^128, the results are infinities.
+ * Sequences may share pages: what one appends the others see, and a slot that two rows of one call are appended to holds
+ * pieces of either.
  * At most 65535 heads and sequences, and 2^29 positions of a sequence, rows and pages. */
 
 /* q and k turned by their positions (RopeCache::forward{,_interleaved}, fusor-ml/fusor/src/composite/rope.rs:284-329; with
@@ -338,7 +340,8 @@ fh_status fh_flash_attention_decode_static(fh_device *dev, int32_t q_dtype, int3
  * position in the cache.  interleaved: pairs are (2j, 2j + 1), otherwise (j, j + n) of n turned pairs.  Products are f32, each
  * rounded on its own, results rounded once to their type.
  * A row whose position has no page, or any of whose axes' positions lies outside the tables, is dropped: neither the
- * pages nor its row of q_out are written.  q_out may be q itself where that is contiguous. */
+ * pages nor its row of q_out are written.  q_out may be q itself where that is contiguous.
+ * Fewer than 2^24 rows. */
 fh_status fh_paged_rope_append(fh_device *dev, int32_t dtype, int32_t kv_dtype, const void *q_dev, int64_t q_st,
                                int64_t q_sh, const void *k_dev, const void *v_dev, int64_t kv_st, int64_t kv_sh, int32_t hq,
                                int32_t hkv, int32_t d, const float *cos_dev, const float *sin_dev, int32_t table_rows,
@@ -350,10 +353,12 @@ fh_status fh_paged_rope_append(fh_device *dev, int32_t dtype, int32_t kv_dtype, 
 /* softmax(q . K^T * scale) . V over the pages, causal: the row of position p sees the positions j <= p of its sequence, with
  * window > 0 only those with j > p - window.  q is [tokens, hq, d] with strides q_st and q_sh (elements), out contiguous
  * [tokens, hq, d]; query head h reads KV head h / (hq / hkv).  A row that sees nothing gets zeros.  scale: 2^-60 and above.
+ * out is memory of its own.
  * max_new: the most rows a sequence has; of sequences with more, the first max_new are computed and the rest left as they
  * were.  With 1 (a decode step) long caches are split over the device and joined in the same launch; with more the rows run on
- * the tiles of a prompt, split over a long cache where they are few, and joined by a second launch.  max_new * hq / hkv is at
- * most 4194240.  max_len: the longest sequence, or 0 where the host does not know; it chooses between forms of the
+ * the tiles of a prompt (a few behind a short cache as single ones do), split over a long cache where they are few, and joined
+ * by a second launch.  max_new * hq / hkv is at most 4194240; seqs * hkv * table_cols * page_size, and as many times as hq / hkv
+ * heads are 16, at most 2^38.  max_len: the longest sequence, or 0 where the host does not know; it chooses between forms of the
  * kernels, whose results differ by their rounding, and nothing else.  Results do not depend on which pages hold a sequence, and
  * are the same bits in every run.  Parts of a split cache meet in scratch memory that the device handle grows: captured calls
  * need an eager one of their size before (prompts that find none run unsplit). */

@@ -249,6 +249,8 @@ extern "C" fh_status fh_paged_rope_append(fh_device *dev, int32_t dtype, int32_t
                               starts_dev, lens_dev, table_dev, table_cols, seqs, tokens, &kv, &rows));
     FH_REQUIRE(k_dev && v_dev, "NULL argument");
     FH_REQUIRE(!q_dev == !q_out_dev, "q and its output come together");
+    FH_REQUIRE(!q_dev || q_dev != q_out_dev || ((hq == 1 || q_sh == d) && (tokens <= 1 || q_st == (int64_t)hq * d)), "q with strides cannot be its own output");
+    FH_REQUIRE(tokens < 1 << 24, "%d rows: a launch takes fewer than 2^24", tokens); // (of 256 threads each, 2^32 in all)
     FH_REQUIRE((cos_dev != nullptr) == (sin_dev != nullptr), "cos and sin come together");
     PagedTurn turn = {};
     if (cos_dev) {
@@ -312,6 +314,9 @@ extern "C" fh_status fh_paged_attention(fh_device *dev, int32_t dtype, int32_t k
     FH_TRY(fh_paged_arguments(dtype, kv_dtype, hq, hkv, d, k_pages_dev, v_pages_dev, page_stride, head_stride, slot_stride, pages, page_size,
                               starts_dev, lens_dev, table_dev, table_cols, seqs, tokens, &kv, &rows));
     FH_REQUIRE(q_dev && out_dev, "NULL argument");
+    FH_REQUIRE(q_dev != out_dev, "q cannot be the output"); // (a row may be read again after it was written)
+    FH_REQUIRE((int64_t)seqs * hkv * ((hq / hkv + 15) / 16) * ((int64_t)table_cols * page_size) <= (int64_t)1 << 38,
+               "%d sequences of %d heads and %d pages of %d positions: more than 2^38 in all", seqs, hkv, table_cols, page_size);
     FH_REQUIRE(scale >= 0x1p-60f && scale < INFINITY, "scale %g", (double)scale);
     FH_REQUIRE(window >= 0 && max_new >= 0 && max_len >= 0, "window %d, max_new %d, max_len %d", window, max_new, max_len);
     FH_REQUIRE(dev, "NULL device");

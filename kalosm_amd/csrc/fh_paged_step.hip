@@ -618,7 +618,7 @@ bool fh_paged_step_whole(const fh_device *dev, int kv_dtype, const PagedCall &ca
     const int64_t most = (int64_t)call.window + call.rows.max_new + TK;
     if (call.window > 0 && most < longest) longest = most;
     const int64_t tiles = (longest + TK - 1) / TK * (call.d > 128 ? 2 : 1), pairs = (int64_t)call.rows.seqs * call.hkv * ((wide + 15) / 16);
-    if (pairs > INT32_MAX) return false; // (workgroups)
+    if (pairs >= 1 << 24) return false; // (workgroups of 256 threads: fewer than 2^32 in all)
     return tiles <= 32 || (tiles <= 48 && 2 * pairs >= dev->compute_units) || (tiles <= 64 && pairs >= dev->compute_units);
 }
 template <typename TX, typename TP>

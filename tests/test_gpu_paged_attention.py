@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from pagedgen import Pages, near, pack, unpack
-from kalosm_amd.fusor import FusorHipError, PagedBatch, Tensor
+from kalosm_amd.fusor import FusorHipError, PagedBatch, PagedKvCache, Tensor
 
 pytestmark = pytest.mark.gpu
 
@@ -404,3 +404,17 @@ def test_scores_that_rise(dev, act, kept, d, new, lens, rise):
     q[:, :, 0] = d ** 0.5 * np.array([1, 0.5, 1, 2])
     p.q = pack(q, act)
     check(dev, p, what=f"{rise} a position")
+
+
+def test_more_pairs_than_workgroups_of_a_launch(dev):
+    """65535 sequences of 260 KV heads, a position each, in pages that they share."""
+    seqs, heads, d, pages = 65535, 260, 8, 64
+    rng = np.random.default_rng(94)
+    v = pack(rng.standard_normal((pages, heads, 16, d)), "f16")
+    kt, vt = (Tensor.from_slice(dev, x, "f16") for x in (v[::-1].copy(), v))
+    cache = PagedKvCache.over(kt, vt)
+    table = (np.arange(seqs) * 7 % pages).astype(np.int32)
+    batch = PagedBatch(Tensor.from_slice(dev, np.ones(seqs, np.int32), "i32"), Tensor.from_slice(dev, table[:, None], "i32"), tokens=seqs)
+    q = Tensor.from_slice(dev, np.full((seqs, heads, d), 0.5, np.float16), "f16")
+    got = q.paged_attention(cache, batch, 0.25).as_slice()
+    assert np.array_equal(got.view(np.uint16), v[table, :, 0].view(np.uint16))

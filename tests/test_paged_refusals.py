@@ -10,7 +10,7 @@ INVALID, UNSUPPORTED = _lib.FH_ERR_INVALID, _lib.FH_ERR_UNSUPPORTED
 P = 4096  # a pointer that is aligned and never followed
 
 ATTENTION = dict(dtype=1, kv_dtype=1, q=P, q_st=512, q_sh=64, hq=8, hkv=2, d=64, scale=0.125, window=0, k=P, v=P, page=2048, head=1024, slot=64,
-                 pages=9, page_size=16, starts=P, lens=P, table=P, cols=4, seqs=2, tokens=5, max_new=3, max_len=0, out=P)
+                 pages=9, page_size=16, starts=P, lens=P, table=P, cols=4, seqs=2, tokens=5, max_new=3, max_len=0, out=2 * P)
 APPEND = dict(dtype=1, kv_dtype=1, q=P, q_st=512, q_sh=64, kr=P, vr=P, kv_st=128, kv_sh=64, hq=8, hkv=2, d=64, cos=P, sin=P, rows=64, pairs=32, positions=None,
               sections=None, axes=1, interleaved=0, k=P, v=P, page=2048, head=1024, slot=64, pages=9, page_size=16, starts=P, lens=P, table=P,
               cols=4, seqs=2, tokens=5, out=P)
@@ -38,7 +38,8 @@ def call(name, base, change):
 
 @pytest.mark.parametrize("change,status,text", SHARED + [
     (dict(q=0), INVALID, "NULL"), (dict(out=0), INVALID, "NULL"), (dict(scale=0.0), INVALID, "scale"), (dict(scale=float("nan")), INVALID, "scale"),
-    (dict(scale=float("inf")), INVALID, "scale"), (dict(window=-1), INVALID, "window"), (dict(max_new=-1), INVALID, "max_new"), (dict(max_len=-1), INVALID, "max_len")])
+    (dict(scale=float("inf")), INVALID, "scale"), (dict(window=-1), INVALID, "window"), (dict(max_new=-1), INVALID, "max_new"), (dict(max_len=-1), INVALID, "max_len"),
+    (dict(out=P), INVALID, "q cannot be"), (dict(seqs=65535, cols=1 << 18), INVALID, "2^38"), (dict(hq=65528, seqs=2048, cols=1 << 14), INVALID, "2^38")])
 def test_attention(change, status, text):
     got, said = call("fh_paged_attention", ATTENTION, change)
     assert got == status and text in said, (got, said)
@@ -47,7 +48,8 @@ def test_attention(change, status, text):
 @pytest.mark.parametrize("change,status,text", SHARED + [
     (dict(kr=0), INVALID, "NULL"), (dict(vr=0), INVALID, "NULL"), (dict(q=0), INVALID, "together"), (dict(out=0), INVALID, "together"), (dict(cos=0), INVALID, "together"),
     (dict(axes=0), INVALID, "axes"), (dict(axes=5), INVALID, "axes"), (dict(axes=2), INVALID, "several axes"), (dict(rows=0), INVALID, "tables"),
-    (dict(pairs=33), INVALID, "sections of 33"), (dict(cos=0, sin=0, positions=P), INVALID, "without tables")])
+    (dict(pairs=33), INVALID, "sections of 33"), (dict(cos=0, sin=0, positions=P), INVALID, "without tables"),
+    (dict(q_st=1024), INVALID, "its own output"), (dict(q_sh=72), INVALID, "its own output"), (dict(tokens=1 << 24), INVALID, "2^24")])
 def test_append(change, status, text):
     got, said = call("fh_paged_rope_append", APPEND, change)
     assert got == status and text in said, (got, said)
