@@ -418,3 +418,19 @@ def test_more_pairs_than_workgroups_of_a_launch(dev):
     q = Tensor.from_slice(dev, np.full((seqs, heads, d), 0.5, np.float16), "f16")
     got = q.paged_attention(cache, batch, 0.25).as_slice()
     assert np.array_equal(got.view(np.uint16), v[table, :, 0].view(np.uint16))
+
+
+@pytest.mark.parametrize("new", [[1, 1], [2, 3], [20, 130]])
+@pytest.mark.parametrize("act,kept", TYPES)
+@pytest.mark.parametrize("d", [64, 200])
+def test_results_at_an_odd_address(dev, new, act, kept, d):
+    p = Pages(13, new, [150, 333], 4, 2, d, 16, act, kept)
+    cache, batch = p.put(dev)
+    n = p.q.size
+    room = Tensor.filled_bytes(dev, (n + 8,), 0xFF, act)
+    q = Tensor.from_slice(dev, p.q, act)
+    q.paged_attention(cache, batch, d ** -0.5, out=Tensor(dev, p.q.shape, act, ptr=room.ptr + 3 * p.q.itemsize))
+    want, bound = p.attention(d ** -0.5)
+    got = unpack(room.as_slice(), act)
+    near(got[3:n + 3].reshape(want.shape), want, bound, f"{act} {d}")
+    assert np.isnan(got[:3]).all() and np.isnan(got[n + 3:]).all()
