@@ -361,11 +361,13 @@ class Tensor:
         positions where that is not 0.  `strides` = (row, head) element strides of a view (of a fused projection's rows,
         say) whose logical shape is self.shape.  The keys and values of the rows themselves must have been appended."""
         tokens, hq, d = self.shape
-        if tokens != batch.tokens or d != cache.head_dim:
-            raise FusorHipError(_lib.FH_ERR_INVALID, f"rows of shape {self.shape} do not match a batch of {batch.tokens} rows "
-                                                     f"and a cache of head_dim {cache.head_dim}")
+        if tokens != batch.tokens or d != cache.head_dim or self.dtype not in _ELEMENTS or self.device is not cache.device:
+            raise FusorHipError(_lib.FH_ERR_INVALID, f"rows of shape {self.shape} ({self.dtype}) do not match a batch of {batch.tokens} rows "
+                                                     f"and a cache of head_dim {cache.head_dim}, on one device")
         if out is None:
             out = Tensor(self.device, self.shape, self.dtype)
+        elif out.shape != self.shape or out.dtype != self.dtype:
+            raise FusorHipError(_lib.FH_ERR_INVALID, f"out is {self.dtype} {self.shape}, not {out.dtype} {out.shape}")
         st, sh = strides or (hq * d, d)
         L = self.device._lib
         status = L.fh_paged_attention(self.device._h, _ELEMENTS[self.dtype], cache.code, self.ptr, st, sh, hq, cache.kv_heads, d,
@@ -616,7 +618,7 @@ class KvCache:
 
 class PagedBatch:
     """Which rows of a call belong to which sequence, and the pages of every sequence: device tensors that the calls read
-    when they run, so a program (or a captured graph) fills in new lengths and pages between them.
+    when they run, so a program (or a captured graph) fills in new lengths and pages between them (other tensors are another batch).
 
     lens [n] i32: positions of every sequence, its new rows among them.  table [n, columns] i32: its pages.  starts [n + 1]
     i32: sequence i has the rows starts[i] .. starts[i + 1] - 1; None: one row each.  tokens: rows of the tensors.  max_new:
@@ -677,9 +679,10 @@ class PagedKvCache:
 
     def _append(self, rope, q, k, v, batch, positions, sections, interleaved, layer, strides, out):
         n, hkv, d = k.shape
-        if k.shape != v.shape or k.dtype != v.dtype or n != batch.tokens or hkv != self.kv_heads or d != self.head_dim:
-            raise FusorHipError(_lib.FH_ERR_INVALID, f"k {k.shape} and v {v.shape} do not match a batch of {batch.tokens} rows and a "
-                                                     f"cache of {self.kv_heads} heads of {self.head_dim}")
+        if k.shape != v.shape or k.dtype != v.dtype or n != batch.tokens or hkv != self.kv_heads or d != self.head_dim \
+                or k.dtype not in _ELEMENTS or k.device is not self.device:
+            raise FusorHipError(_lib.FH_ERR_INVALID, f"k {k.shape} ({k.dtype}) and v {v.shape} ({v.dtype}) do not match a batch of {batch.tokens} "
+                                                     f"rows and a cache of {self.kv_heads} heads of {self.head_dim}, on one device")
         hq = hkv
         if q is not None:
             hq = q.shape[1]
@@ -687,6 +690,8 @@ class PagedKvCache:
                 raise FusorHipError(_lib.FH_ERR_INVALID, f"q {q.shape} {q.dtype} does not match k {k.shape} {k.dtype}")
             if out is None:
                 out = Tensor(self.device, q.shape, q.dtype)
+            elif out.shape != q.shape or out.dtype != q.dtype:
+                raise FusorHipError(_lib.FH_ERR_INVALID, f"out is {q.dtype} {q.shape}, not {out.dtype} {out.shape}")
         cos, sin, rows, pairs, axes, sec = None, None, 0, 0, 1, None
         if rope is not None:
             cos, sin, (rows, pairs) = rope.cos.ptr, rope.sin.ptr, rope.cos.shape

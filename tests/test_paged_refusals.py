@@ -5,6 +5,7 @@ import ctypes as C
 import pytest
 
 from kalosm_amd import _lib
+from kalosm_amd.fusor import FusorHipError, PagedBatch, PagedKvCache, RopeCache, Tensor
 
 INVALID, UNSUPPORTED = _lib.FH_ERR_INVALID, _lib.FH_ERR_UNSUPPORTED
 P = 4096  # a pointer that is aligned and never followed
@@ -68,3 +69,41 @@ def test_what_is_right_wants_its_device():
         for change in (dict(page=2048, head=64, slot=128), dict(dtype=0), dict(dtype=0, kv_dtype=2), dict(dtype=2, kv_dtype=2), dict(hkv=1, page=1024, head=64)):
             got, said = call(name, base, change)
             assert got == INVALID and "device" in said, (change, said)
+
+
+def test_tensors_that_do_not_match():
+    """Wrong shapes, types and devices on the way in, on devices that are none (nothing here gets as far as a call)."""
+    class Nowhere:
+        _lib, _h = _lib.load(), None
+
+        def alloc(self, size):
+            return P
+
+        def free(self, ptr):
+            pass
+
+    here, there = Nowhere(), Nowhere()
+
+    def t(*shape, dtype="f16", device=here):
+        return Tensor(device, shape, dtype, ptr=P)
+
+    cache, batch = PagedKvCache.over(t(9, 2, 16, 64), t(9, 2, 16, 64)), PagedBatch(t(3, dtype="i32"), t(3, 4, dtype="i32"))
+    q, k = t(3, 8, 64), t(3, 2, 64)
+    rope = RopeCache.__new__(RopeCache)
+    rope.cos, rope.sin = t(32, 32, dtype="f32"), t(32, 32, dtype="f32")
+    for text, call in (("out is", lambda: q.paged_attention(cache, batch, 0.1, out=t(3, 8, 32))), ("out is", lambda: q.paged_attention(cache, batch, 0.1, out=t(3, 8, 64, dtype="f32"))),
+                       ("match a batch", lambda: t(4, 8, 64).paged_attention(cache, batch, 0.1)), ("match a batch", lambda: t(3, 8, 32).paged_attention(cache, batch, 0.1)),
+                       ("match a batch", lambda: t(3, 8, 64, dtype="i32").paged_attention(cache, batch, 0.1)),
+                       ("one device", lambda: t(3, 8, 64, device=there).paged_attention(cache, batch, 0.1)), ("one device", lambda: cache.append(t(3, 2, 64, device=there), k, batch)),
+                       ("match a batch", lambda: cache.append(k, t(3, 2, 64, dtype="f32"), batch)), ("match a batch", lambda: cache.append(t(3, 1, 64), t(3, 1, 64), batch)),
+                       ("match a batch", lambda: cache.append(t(3, 2, 64, dtype="i32"), t(3, 2, 64, dtype="i32"), batch)),
+                       ("does not match k", lambda: rope.forward_paged(t(2, 8, 64), k, k, cache, batch)), ("out is", lambda: rope.forward_paged(q, k, k, cache, batch, out=t(3, 8, 64, dtype="f32"))),
+                       ("positions are", lambda: rope.forward_paged(q, k, k, cache, batch, positions=t(1, 2, dtype="i32"))), ("layer 1", lambda: cache.append(k, k, batch, layer=1))):
+        with pytest.raises(FusorHipError, match=text):
+            call()
+    with pytest.raises(FusorHipError, match="lens is i32"):
+        PagedBatch(t(2, dtype="i32"), t(3, 4, dtype="i32"))
+    with pytest.raises(FusorHipError, match="starts"):
+        PagedBatch(t(3, dtype="i32"), t(3, 4, dtype="i32"), t(4, dtype="i32"))
+    with pytest.raises(FusorHipError, match="pages of shapes"):
+        PagedKvCache.over(t(9, 2, 16, 64), t(9, 2, 16, 32))
