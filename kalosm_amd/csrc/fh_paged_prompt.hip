@@ -8,6 +8,9 @@
 // A page's 16 positions are one scalar address: requests add a lane's constant offset.
 // grid (KV heads, blocks of rows - the last, longest ones first -, sequences x parts).  With fewer workgroups than compute units the
 // positions are split over `parts` workgroups, whose sums go to scratch memory in f32 and are added up by a second launch.
+// Measured (32 / 8 heads of 128): 8192 tokens of f16 605 to 645 us by the card, 855 to 910 TFLOP/s, the matrix cores busy 44 % of the cycles; 8 sequences of
+// 184 to 512 behind up to 4001, bf16, 179 us, 740; 33 behind 65536, f16, 90 us, 3.0 TB/s (a workgroup has one step of 64 KB on its way, which takes 2.3 us
+// whatever the number of rows).  2 x 2049, window 1024, 16 / 4 heads of 64, f32: 104 us, 110 TFLOP/s.
 //
 // Positions that a row does not see have weight 0, whatever lies there: scores are replaced, and where a row's sums end up infinite or NaN and a position in its
 // tiles that some row does not see has an infinity or a NaN - 0 times that is NaN - the row is worked out again in f32 over what it sees (pp_mend): one at a
