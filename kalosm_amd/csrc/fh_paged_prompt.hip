@@ -733,6 +733,9 @@ template <typename T> static fh_status pp_same(fh_device *dev, PpArgs a, int64_t
     if (a.c.d > 128) return pp_planes<T, T, 256>(dev, a, longest);
     const int64_t rows = (int64_t)a.c.rows.max_new * (a.c.hq / a.c.hkv), pairs = (int64_t)a.c.hkv * a.c.rows.seqs;
     const int64_t wgs = pairs * ((rows + 127) / 128);
+    // Two groups of four wavefronts share a workgroup's positions while no more than two workgroups of four would have come to a compute unit (32 / 8 heads of 128, us,
+    // two groups / one: 1024 behind 4000 101 / 131, 33 behind 65536 91 / 117, 2048 alone 58 / 62, behind 4000 193 / 186; 4096 alone 187 / 176, 8192 670 / 604,
+    // 8 of 512 behind 4001 211 / 173).
     const bool halves = wgs <= 2 * dev->compute_units && longest > 128;
     a.sorted = wgs > dev->compute_units;
     pp_parts(dev, a.c, wgs, longest, 128, 3, &a);
