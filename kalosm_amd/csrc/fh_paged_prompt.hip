@@ -120,8 +120,8 @@ __device__ __forceinline__ void pp_again(const PpArgs &a, int part, int seq, con
     if (a.parts > 1 && lane == 0) a.stats[2 * where] = m, a.stats[2 * where + 1] = l;
 }
 // The rows of a wavefront, first .. first + 31 of the sequence's `rows`, whose sums are not finite, again, where positions from .. to have an infinity or a NaN
-// among the values that not all of them see.  And rows whose scores' largest, m, is of 2^25 or more, next to f16: what 14 - m is rounded by, and m itself, takes
-// weights out of f16's range.
+// among the values that not all of them see.  And rows whose scores' largest, m, is of 2^25 or more: what m is rounded by (and 14 - m, next to f16) goes into
+// every weight's exponent, and takes it out of f16's range from there on, of f32's from 2^31.
 template <typename TX, typename TP, int D>
 __device__ __forceinline__ void pp_mend(const PpArgs &a, int part, int seq, const PagedSeq &s, const PpRow &x, int first, int rows, int kh, int group, int from, int to, bool holed,
                                         float m, float l, const floatx16 (&acc)[D / 32]) {
@@ -132,7 +132,7 @@ __device__ __forceinline__ void pp_mend(const PpArgs &a, int part, int seq, cons
         for (int r = 0; r < 16; r++) sum = fmaf(0.f, acc[dt][r], sum);
     uint64_t bad = __ballot(!(sum == 0.f));
     bad = (bad | bad >> 32) & 0xFFFFFFFFu;
-    uint64_t rounded = __ballot(__is_same(TP, fh_half) && fabsf(m) >= 0x1p25f && fabsf(m) < INFINITY);
+    uint64_t rounded = __ballot(fabsf(m) >= 0x1p25f && fabsf(m) < INFINITY);
     rounded = (rounded | rounded >> 32) & 0xFFFFFFFFu;
     if (!(bad | rounded)) return;
     // what lies behind the first row's end, and in front of the last one's beginning

@@ -385,12 +385,14 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
 #pragma unroll
             for (int h = 0; h < HALVES; h++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) p[h][i] = fmaf(st[h][i], sc2, sub);
-            if (F16 && __any(fabsf(ref) >= 0x1p25f)) // what 14 - ref is rounded by, and ref itself, would take weights out of f16's range
+                for (int i = 0; i < 4; i++) p[h][i] = F32 ? st[h][i] * sc2 + sub : fmaf(st[h][i], sc2, sub);
+            // From a maximum of 2^25 on, what ref and sub are rounded by would go into the exponents, and take weights out of f16's range (from 2^31: f32's): scores
+            // rounded as the maximum was, as those of f32 pages always are.
+            if (!F32 && __any(fabsf(ref) >= 0x1p25f))
 #pragma unroll
                 for (int h = 0; h < HALVES; h++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) p[h][i] = st[h][i] * sc2 - ref + 14.f;
+                    for (int i = 0; i < 4; i++) p[h][i] = st[h][i] * sc2 - ref + (F16 ? 14.f : 0.f);
 #pragma unroll
             for (int h = 0; h < HALVES; h++)
 #pragma unroll

@@ -3,7 +3,7 @@ and several (tiles of a prompt); slots that nothing may see hold NaN in every ca
 import numpy as np
 import pytest
 
-from pagedgen import Pages, near, pack, unpack
+from pagedgen import HALF_STEP, SMALLEST, Pages, near, pack, unpack
 from kalosm_amd.fusor import FusorHipError, PagedBatch, PagedKvCache, Tensor
 
 pytestmark = pytest.mark.gpu
@@ -434,3 +434,30 @@ def test_results_at_an_odd_address(dev, new, act, kept, d):
     got = unpack(room.as_slice(), act)
     near(got[3:n + 3].reshape(want.shape), want, bound, f"{act} {d}")
     assert np.isnan(got[:3]).all() and np.isnan(got[n + 3:]).all()
+
+
+@pytest.mark.parametrize("act,kept", [("f32", "f32"), ("bf16", "bf16"), ("f32", "bf16")])
+@pytest.mark.parametrize("d", [64, 128, 200])
+@pytest.mark.parametrize("new,lens", [([1] * 24, [100] * 24), ([1, 1], [9000, 3000]), ([4] * 9, [60] * 9), ([300, 100], [300, 900]), ([3], [5000])])
+def test_scores_past_the_exponents_of_their_steps(dev, act, kept, d, new, lens):
+    """The same up to scores of 2^76, where they are rounded by 2^52: a weight's exponent must not have that in it."""
+    p = Pages(95, new, lens, 4, 2, d, 16, act, kept)
+    rng = np.random.default_rng(96)
+    values = (np.arange(0x4F00, 0x5F00, dtype=np.uint32) << 16).view(np.float32)  # 2^31 to 2^63, each 1 / 256 or more above the one before
+    k = np.zeros(p.k.shape)
+    k[:, :, :, 0] = 1
+    for i, n in enumerate(lens):
+        at = rng.permutation(n)[:2000]
+        k[p.table[i, at // 16], :, at % 16, 0] = rng.permutation(values)[:len(at), None]
+    p.k = pack(k, kept)
+    q = np.zeros(p.q.shape)
+    q[:, :, 0] = rng.uniform(4000, 60000, (p.tokens, 4))
+    p.q = pack(q, act)
+    got = run(dev, p)
+    want = np.zeros_like(got)
+    for row, i, last in p.rows():
+        j = np.arange(last + 1)
+        top = int(np.argmax(k[p.table[i, j // 16], 0, j % 16, 0]))
+        want[row] = np.repeat(unpack(p.v[p.table[i, top // 16], :, top % 16], kept), 2, 0)
+    weight = HALF_STEP[kept] if act == kept else 2.0 ** -22
+    near(got, want, 1.01 * (HALF_STEP[act] + weight + 2.0 ** -22) * np.abs(want) + SMALLEST[act], f"{act} {kept} {d} {new[:3]}")
