@@ -352,7 +352,7 @@ fh_status fh_paged_rope_append(fh_device *dev, int32_t dtype, int32_t kv_dtype, 
                                int32_t table_cols, int32_t seqs, int32_t tokens, void *q_out_dev);
 /* softmax(q . K^T * scale) . V over the pages, causal: the row of position p sees the positions j <= p of its sequence, with
  * window > 0 only those with j > p - window.  q is [tokens, hq, d] with strides q_st and q_sh (elements), out contiguous
- * [tokens, hq, d]; query head h reads KV head h / (hq / hkv).  A row that sees nothing gets zeros.  scale: 2^-60 and above.
+ * [tokens, hq, d]; query head h reads KV head h / (hq / hkv).  A row that sees nothing gets zeros.  scale: 2^-60 to 2^60.
  * out is memory of its own.
  * max_new: the most rows a sequence has; of sequences with more, the first max_new are computed and the rest left as they
  * were.  With 1 (a decode step) long caches are split over the device and joined in the same launch; with more the rows run on

@@ -318,7 +318,7 @@ extern "C" fh_status fh_paged_attention(fh_device *dev, int32_t dtype, int32_t k
     FH_REQUIRE(q_dev != out_dev, "q cannot be the output"); // (a row may be read again after it was written)
     FH_REQUIRE((int64_t)seqs * hkv * ((hq / hkv + 15) / 16) * ((int64_t)table_cols * page_size) <= (int64_t)1 << 38,
                "%d sequences of %d heads and %d pages of %d positions: more than 2^38 in all", seqs, hkv, table_cols, page_size);
-    FH_REQUIRE(scale >= 0x1p-60f && scale < INFINITY, "scale %g", (double)scale);
+    FH_REQUIRE(scale >= 0x1p-60f && scale <= 0x1p60f, "scale %g", (double)scale);
     FH_REQUIRE(window >= 0 && max_new >= 0 && max_len >= 0, "window %d, max_new %d, max_len %d", window, max_new, max_len);
     FH_REQUIRE(dev, "NULL device");
     if (!tokens || !seqs || !max_new) return FH_OK;

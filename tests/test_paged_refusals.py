@@ -40,7 +40,7 @@ def call(name, base, change):
 @pytest.mark.parametrize("change,status,text", SHARED + [
     (dict(q=0), INVALID, "NULL"), (dict(out=0), INVALID, "NULL"), (dict(scale=0.0), INVALID, "scale"), (dict(scale=float("nan")), INVALID, "scale"),
     (dict(scale=float("inf")), INVALID, "scale"), (dict(window=-1), INVALID, "window"), (dict(max_new=-1), INVALID, "max_new"), (dict(max_len=-1), INVALID, "max_len"),
-    (dict(out=P), INVALID, "q cannot be"), (dict(seqs=65535, cols=1 << 18), INVALID, "2^38"), (dict(hq=65528, seqs=2048, cols=1 << 14), INVALID, "2^38")])
+    (dict(out=P), INVALID, "q cannot be"), (dict(scale=2.0 ** 61), INVALID, "scale"), (dict(scale=2.0 ** -61), INVALID, "scale"), (dict(seqs=65535, cols=1 << 18), INVALID, "2^38"), (dict(hq=65528, seqs=2048, cols=1 << 14), INVALID, "2^38")])
 def test_attention(change, status, text):
     got, said = call("fh_paged_attention", ATTENTION, change)
     assert got == status and text in said, (got, said)
