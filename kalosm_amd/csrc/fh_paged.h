@@ -7,6 +7,11 @@ typedef __bf16 fh_bf;
 
 enum { FH_PAGED_BF16 = FH_DECODER_BF16, FH_PAGED_MAX = 1 << 29 /* positions of a sequence */ };
 
+// From a maximum m of this size on, in the log2 domain, a weight's exponent is (score rounded as m was - m) + 14 next to f16, without the 14 next to
+// other types; below it one fma: score + (14 - m).  What m and 14 - m are rounded by is in the latter, and 14 - m is rounded by more than m where it lies above a power
+// of two that |m| is below: below 2^22 by 2^-3 and 2^-2 at most, so weights that start at 2^14, or 2^15.5 in prompts, stay below f16's 2^16.
+#define PAGED_FAR 0x1p22f
+
 struct PagedKv {
     const char *k, *v;
     int64_t page, head, slot; // strides in bytes, K and V alike

@@ -386,9 +386,8 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
             for (int h = 0; h < HALVES; h++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) p[h][i] = F32 ? st[h][i] * sc2 + sub : fmaf(st[h][i], sc2, sub);
-            // From a maximum of 2^25 on, what ref and sub are rounded by would go into the exponents, and take weights out of f16's range (from 2^31: f32's): scores
-            // rounded as the maximum was, as those of f32 pages always are.
-            if (!F32 && __any(fabsf(ref) >= 0x1p25f))
+            // Scores rounded as the maximum was, as those of f32 pages always are.
+            if (!F32 && __any(fabsf(ref) >= PAGED_FAR))
 #pragma unroll
                 for (int h = 0; h < HALVES; h++)
 #pragma unroll
