@@ -120,11 +120,10 @@ __device__ __forceinline__ void pp_again(const PpArgs &a, int part, int seq, con
     if (a.parts > 1 && lane == 0) a.stats[2 * where] = m, a.stats[2 * where + 1] = l;
 }
 // The rows of a wavefront, first .. first + 31 of the sequence's `rows`, whose sums are not finite, again, where positions from .. to have an infinity or a NaN
-// among the values that not all of them see.  And rows whose scores' largest, m, is of 2^25 or more: what m is rounded by (and 14 - m, next to f16) goes into
-// every weight's exponent, and takes it out of f16's range from there on, of f32's from 2^31.
+// among the values that not all of them see.
 template <typename TX, typename TP, int D>
 __device__ __forceinline__ void pp_mend(const PpArgs &a, int part, int seq, const PagedSeq &s, const PpRow &x, int first, int rows, int kh, int group, int from, int to, bool holed,
-                                        float m, float l, const floatx16 (&acc)[D / 32]) {
+                                        float l, const floatx16 (&acc)[D / 32]) {
     float sum = 0.f * l; // (of 0 times everything)
 #pragma unroll
     for (int dt = 0; dt < D / 32; dt++)
@@ -132,9 +131,7 @@ __device__ __forceinline__ void pp_mend(const PpArgs &a, int part, int seq, cons
         for (int r = 0; r < 16; r++) sum = fmaf(0.f, acc[dt][r], sum);
     uint64_t bad = __ballot(!(sum == 0.f));
     bad = (bad | bad >> 32) & 0xFFFFFFFFu;
-    uint64_t rounded = __ballot(fabsf(m) >= 0x1p25f && fabsf(m) < INFINITY);
-    rounded = (rounded | rounded >> 32) & 0xFFFFFFFFu;
-    if (!(bad | rounded)) return;
+    if (!bad) return;
     // what lies behind the first row's end, and in front of the last one's beginning
     const PagedKv &kv = a.c.kv;
     const int lane = threadIdx.x & 63, pieces = a.c.d * (int)sizeof(TP) / 16;
@@ -156,8 +153,7 @@ __device__ __forceinline__ void pp_mend(const PpArgs &a, int part, int seq, cons
             for (int e = 0; e < 16 / (int)sizeof(TP); e++) wild |= !(0.f * (float)v[e] == 0.f);
         }
     }
-    bad = __any(wild) ? bad | rounded : rounded;
-    if (!bad) return;
+    if (!__any(wild)) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // what was stored before
     for (int i = 0; i < 32; i++)
         if (bad >> i & 1 && first + i < rows) pp_again<TX, TP>(a, part, seq, s, first + i, kh, group, from, to);
@@ -337,7 +333,15 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
                 for (int r = 0; r < 16; r++) acc[dt][r] *= alpha;
         }
-        const float m_sub = (F16 ? 14.f : 0.f) - (m_run == -INFINITY ? 0.f : m_run); // weights of f16 are 2^14 times what they are: 2^-39 of the largest still counts
+        const float ref = m_run == -INFINITY ? 0.f : m_run;
+        float by = sc2, m_sub = (F16 ? 14.f : 0.f) - ref; // weights of f16 are 2^14 times what they are: 2^-39 of the largest still counts
+        if (__any(fabsf(ref) >= PAGED_FAR)) {
+            by = 1.f, m_sub = F16 ? 14.f : 0.f;
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) st[kt][r] = st[kt][r] * sc2 - ref;
+        }
         requests(it);
         __builtin_amdgcn_sched_barrier(0);
         if (!last) scores(it + 1, next);
@@ -349,7 +353,7 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(2, 2))
             for (int s2 = 0; s2 < 2; s2++)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(st[kt][8 * s2 + e], sc2, m_sub));
+                    const float p = __builtin_amdgcn_exp2f(fmaf(st[kt][8 * s2 + e], by, m_sub));
                     ps += p;
                     pb[kt][s2][e] = (T)p;
                 }
@@ -421,7 +425,7 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(2, 2))
     if (KS == 2 && kset == 1) return;
     l_run = ap_swap32_sum(l_run);
     if (r < s.rows * group) pp_store<T, D>(a, part, s, x, kh, group, g, m_run, l_run, acc);
-    pp_mend<T, T, D>(a, part, seq, s, x, r0 + (wave % QW) * 32, s.rows * group, kh, group, span.base, span.base + steps * KS * BN - 1, holed, m_run, l_run, acc);
+    pp_mend<T, T, D>(a, part, seq, s, x, r0 + (wave % QW) * 32, s.rows * group, kh, group, span.base, span.base + steps * KS * BN - 1, holed, l_run, acc);
 }
 
 // ---------------------------------------------------------------- every other type and head_dim
@@ -601,11 +605,17 @@ __global__ __launch_bounds__(256) void k_paged_planes(PpArgs a) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) acc[dt][r] *= alpha;
         }
-        const float m_sub = (F16 ? 14.f : 0.f) - (m_run == -INFINITY ? 0.f : m_run); // (weights of f16: 2^14 times what they are)
+        const float ref = m_run == -INFINITY ? 0.f : m_run;
+        float by = sc2, m_sub = (F16 ? 14.f : 0.f) - ref; // (weights of f16: 2^14 times what they are)
+        if (__any(fabsf(ref) >= PAGED_FAR)) {
+            by = 1.f, m_sub = F16 ? 14.f : 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) st[r] = st[r] * sc2 - ref;
+        }
         vec8 pb[QT][2];
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-            float p = __builtin_amdgcn_exp2f(fmaf(st[r], sc2, m_sub));
+            float p = __builtin_amdgcn_exp2f(fmaf(st[r], by, m_sub));
             l_run += p;
 #pragma unroll
             for (int u = 0; u < QT; u++) {
@@ -630,7 +640,7 @@ __global__ __launch_bounds__(256) void k_paged_planes(PpArgs a) {
     }
     l_run = ap_swap32_sum(l_run);
     if (r < s.rows * group) pp_store<TX, DP>(a, part, s, x, kh, group, g, m_run, l_run, acc);
-    pp_mend<TX, TP, DP>(a, part, seq, s, x, r0 + wave * 32, s.rows * group, kh, group, span.base, span.base + span.steps * BN - 1, holed, m_run, l_run, acc);
+    pp_mend<TX, TP, DP>(a, part, seq, s, x, r0 + wave * 32, s.rows * group, kh, group, span.base, span.base + span.steps * BN - 1, holed, l_run, acc);
 }
 
 // ---------------------------------------------------------------- the parts together

@@ -10,6 +10,7 @@ pytestmark = pytest.mark.gpu
 
 TYPES = [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "f16"), ("f32", "bf16")]
 STEPS = [([1] * 24, [100] * 24), ([1] * 3, [2000, 9000, 500]), ([4] * 9, [60] * 9)]
+PROMPTS = [([70] * 8, [300] * 8), ([60] * 3, [128] * 3), ([20], [3000])]
 LN2 = 0.6931471824645996  # times 1.4426950408889634 this is 1 in f32: scores are whole numbers to base 2
 
 
@@ -65,3 +66,34 @@ def whole_scores(dev, act, kept, d, new, lens):
 @pytest.mark.parametrize("new,lens", STEPS)
 def test_steps_at_whole_scores(dev, act, kept, d, new, lens):
     whole_scores(dev, act, kept, d, new, lens)
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 200])
+@pytest.mark.parametrize("new,lens", PROMPTS)
+def test_prompts_at_whole_scores(dev, act, kept, d, new, lens):
+    whole_scores(dev, act, kept, d, new, lens)
+
+
+@pytest.mark.parametrize("act,kept", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 200])
+@pytest.mark.parametrize("new,lens,low", [([1] * 24, [100] * 24, 64), ([1] * 2, [9000, 3000], 2048), ([4] * 9, [60] * 9, 48), ([60, 30], [128, 128], 64), ([130, 40], [400, 700], 256),
+                                          ([20], [5000], 4096), ([300, 40], [2348, 2100], 2048)])
+def test_the_first_positions_far_below(dev, act, kept, d, new, lens, low):
+    """The first `low` positions score -2^25 and less (next to f16; else -2^37 and less), the others as usual: weights of the first are 0, and the result is that of
+    the others alone, whatever the first tiles' maxima were rounded by."""
+    p = Pages(7, new, lens, 8, 2, d, 16, act, kept)
+    rng = np.random.default_rng(17)
+    k, q = unpack(p.k, kept), unpack(p.q, act)
+    far = 3.5e4 if kept == "f16" else 2.0 ** 21
+    for i, n in enumerate(lens):
+        pos = np.arange(n)
+        at = k[p.table[i, pos // 16], :, pos % 16]
+        at[..., 0] = np.where(pos < low, -(10000.0 if kept == "f16" else 2.0 ** 20), 0)[:, None]
+        k[p.table[i, pos // 16], :, pos % 16] = at
+    q[:, :, 0] = far * rng.uniform(0.75, 1.5, q.shape[:2])
+    p.k, p.q = pack(k, kept), pack(q, act)
+    got = run(dev, p, 0.125)
+    p.table[:, :low // 16] = -1  # (of the oracle: positions that are not there)
+    want, bound = p.attention(0.125)
+    near(got, want, bound, f"{act}/{kept} {d} {new[:2]}")
