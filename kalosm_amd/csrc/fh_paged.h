@@ -49,6 +49,14 @@ __device__ __forceinline__ PagedSeq paged_seq_scalar(const PagedRows &r, int shi
     return r.starts ? paged_seq(r, shift, len, paged_scalar(r.starts, i), paged_scalar(r.starts, i + 1)) : paged_seq(r, shift, len, i, i + 1);
 }
 
+// The scale of scores whose row is taken 2^ex times as large.  It stays a normal number - ex is no larger than that allows, and scores of smaller rows do not tell
+// positions apart: they are below 2^(15 + 16 + 8 - 126) - and finite: where it would not be, scores are 0 or, of the smallest key, 2^(14 - 24 + 128) apart.
+__device__ __forceinline__ float paged_brought(float scale, int &ex) {
+    const int most = __builtin_amdgcn_frexp_expf(scale) + 125;
+    ex = ex < most ? ex : most;
+    return fminf(ldexpf(scale, -ex), 0x1.fffffep127f);
+}
+
 // One row and head by a wavefront, over the positions from .. to: what the tiles are checked against where they end up infinite or NaN (an infinity or a NaN
 // among values that a neighbour sees and this row does not, terms of an infinite f32).  A key a lane for the scores; o[e]: value lane + 64 e.  m is in
 // the log2 domain, weights are 2^shift times what they are.

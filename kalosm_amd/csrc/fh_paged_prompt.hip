@@ -467,8 +467,7 @@ __global__ __launch_bounds__(256) void k_paged_planes(PpArgs a) {
                     for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf((float)qp[16 * ks + e]));
             most = ap_swap32_max(most);
             if (most > 0.f && most < INFINITY) ex = 15 - __builtin_amdgcn_frexp_expf(most);
-            ex = ex < 60 ? ex : 60; // (below 2^-45 nothing is left to tell scores apart, and the scale must not vanish)
-            sc2 = ldexpf(sc2, -ex);
+            sc2 = paged_brought(sc2, ex);
         }
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ks++) {

@@ -301,8 +301,7 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
                 most = ps_rows_max(most);
                 int ex = 0;
                 if (most > 0.f && most < INFINITY) ex = 15 - __builtin_amdgcn_frexp_expf(most);
-                ex = ex < 60 ? ex : 60; // (below 2^-45 nothing is left to tell scores apart, and the scale must not vanish)
-                sc2 = ldexpf(sc2, -ex);
+                sc2 = paged_brought(sc2, ex);
 #pragma unroll
                 for (int s = 0; s < KL; s++)
 #pragma unroll
