@@ -81,9 +81,9 @@ __device__ __forceinline__ void paged_again(const TX *q, int d, float sc2, float
                     uint4 w[sizeof(TP) / 2];
                     for (int i = 0; i < (int)sizeof(TP) / 2; i++) w[i] = ((const uint4 *)(kv.k + at + e * (int)sizeof(TP)))[i];
                     __builtin_memcpy(x, w, sizeof(x));
-                    for (int i = 0; i < 8; i++) y = fmaf((float)q[e + i], (float)x[i], y);
+                    for (int i = 0; i < 8; i++) y = fmaf((float)q[e + i] * 0x1p-24f, (float)x[i], y); // (f16 keys next to f32 rows: 2^127 * 2^16 * 256)
                 }
-                y *= sc2;
+                y *= sc2 * 0x1p24f;
             }
         }
         float mx = y;

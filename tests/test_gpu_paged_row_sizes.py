@@ -54,3 +54,28 @@ def test_scores_of_zero_beside_the_largest(dev, d, new, lens, sign):
         x = v[p.table[i, j // 16], :, j % 16]
         o, mass, whole = (np.repeat(y, 2, 0) for y in (x.mean(0), np.abs(x).mean(0), np.abs(x).sum(0)))
         near(got[row], o, attention_bound(o, mass, whole, 0.0, last + 1, d, "f32", "f16"), f"row {row}")
+
+
+@pytest.mark.parametrize("d", [64, 128, 200])
+@pytest.mark.parametrize("new,lens", [([4] * 9, [60] * 9), ([70, 20], [300, 90]), ([20], [3000])])
+def test_large_rows_in_front_of_what_they_do_not_see(dev, d, new, lens):
+    """q . k of 2^129 to 2^142 at a scale of 2^-60, and V with infinities where the last row alone looks: the others have the values of their largest key, by the tiles
+    and where they are worked out again.  Keys are 2^-10 of themselves apart and more, scores 2^56 and more: the largest has all of the weight."""
+    p = Pages(9, new, lens, 4, 2, d, 16, "f32", "f16")
+    rng = np.random.default_rng(10)
+    values = np.arange(0x4400, 0x7B00, dtype=np.uint16).view(np.float16).astype(np.float64)  # 4 to 57344
+    v, k = unpack(p.v, "f16"), np.zeros(p.k.shape)
+    for i, n in enumerate(lens):
+        pos = np.arange(n)
+        k[p.table[i, pos // 16], :, pos % 16, 5] = rng.permutation(values)[:n, None]
+        v[p.table[i, (n - 1) // 16], :, (n - 1) % 16, 1] = np.inf
+    p.k, p.v, p.q = pack(k, "f16"), pack(v, "f16"), pack(np.full(p.q.shape, 2.0 ** 127), "f32")
+    got = run(dev, p, 2.0 ** -60)
+    for row, i, last in p.rows():
+        j = np.arange(last + 1)
+        if last + 1 == lens[i]:
+            assert not np.isfinite(got[row, :, 1]).any()
+            continue
+        top = int(np.argmax(k[p.table[i, j // 16], 0, j % 16, 5]))
+        o = np.repeat(v[p.table[i, top // 16], :, top % 16], 2, 0)
+        near(got[row], o, attention_bound(o, np.abs(o), 0 * o, 0.0, last + 1, d, "f32", "f16"), f"row {row}")
