@@ -361,13 +361,13 @@ class Tensor:
         positions where that is not 0.  `strides` = (row, head) element strides of a view (of a fused projection's rows,
         say) whose logical shape is self.shape.  The keys and values of the rows themselves must have been appended."""
         tokens, hq, d = self.shape
-        if tokens != batch.tokens or d != cache.head_dim or self.dtype not in _ELEMENTS or self.device is not cache.device:
+        if tokens != batch.tokens or d != cache.head_dim or self.dtype not in _ELEMENTS or self.device is not cache.device or batch.device is not cache.device:
             raise FusorHipError(_lib.FH_ERR_INVALID, f"rows of shape {self.shape} ({self.dtype}) do not match a batch of {batch.tokens} rows "
                                                      f"and a cache of head_dim {cache.head_dim}, on one device")
         if out is None:
             out = Tensor(self.device, self.shape, self.dtype)
-        elif out.shape != self.shape or out.dtype != self.dtype:
-            raise FusorHipError(_lib.FH_ERR_INVALID, f"out is {self.dtype} {self.shape}, not {out.dtype} {out.shape}")
+        elif out.shape != self.shape or out.dtype != self.dtype or out.device is not self.device:
+            raise FusorHipError(_lib.FH_ERR_INVALID, f"out is {self.dtype} {self.shape} of the rows' device, not {out.dtype} {out.shape}")
         st, sh = strides or (hq * d, d)
         L = self.device._lib
         status = L.fh_paged_attention(self.device._h, _ELEMENTS[self.dtype], cache.code, self.ptr, st, sh, hq, cache.kv_heads, d,
@@ -628,11 +628,11 @@ class PagedBatch:
                  max_new: Optional[int] = None, max_len: int = 0):
         n, cols = table.shape
         for what, t, shape in (("lens", lens, (n,)), ("table", table, (n, cols)), ("starts", starts, (n + 1,))):
-            if t is not None and (t.dtype != "i32" or t.shape != shape):
-                raise FusorHipError(_lib.FH_ERR_INVALID, f"{what} is i32 {shape}, not {t.dtype} {t.shape}")
+            if t is not None and (t.dtype != "i32" or t.shape != shape or t.device is not table.device):
+                raise FusorHipError(_lib.FH_ERR_INVALID, f"{what} is i32 {shape} of the table's device, not {t.dtype} {t.shape}")
         if starts is not None and tokens is None:
             raise FusorHipError(_lib.FH_ERR_INVALID, "a batch with starts needs its number of rows")
-        self.lens, self.table, self.starts = lens, table, starts
+        self.device, self.lens, self.table, self.starts = table.device, lens, table, starts
         self.tokens = n if tokens is None else int(tokens)
         self.max_new = (1 if starts is None else self.tokens) if max_new is None else int(max_new)
         self.max_len = int(max_len)
@@ -658,8 +658,8 @@ class PagedKvCache:
 
     def _over(self, k: Tensor, v: Tensor) -> None:
         shape = k.shape if len(k.shape) == 5 else (1, *k.shape)
-        if len(shape) != 5 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _ELEMENTS:
-            raise FusorHipError(_lib.FH_ERR_INVALID, f"pages of shapes {k.shape}, {v.shape} and types {k.dtype}, {v.dtype}")
+        if len(shape) != 5 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _ELEMENTS or v.device is not k.device:
+            raise FusorHipError(_lib.FH_ERR_INVALID, f"pages of shapes {k.shape}, {v.shape} and types {k.dtype}, {v.dtype}, on one device")
         self.device, self.k, self.v, self.dtype, self.code = k.device, k, v, k.dtype, _ELEMENTS[k.dtype]
         self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = shape
         row = self.page_size * self.head_dim
@@ -680,25 +680,27 @@ class PagedKvCache:
     def _append(self, rope, q, k, v, batch, positions, sections, interleaved, layer, strides, out):
         n, hkv, d = k.shape
         if k.shape != v.shape or k.dtype != v.dtype or n != batch.tokens or hkv != self.kv_heads or d != self.head_dim \
-                or k.dtype not in _ELEMENTS or k.device is not self.device:
+                or k.dtype not in _ELEMENTS or k.device is not self.device or v.device is not self.device or batch.device is not self.device:
             raise FusorHipError(_lib.FH_ERR_INVALID, f"k {k.shape} ({k.dtype}) and v {v.shape} ({v.dtype}) do not match a batch of {batch.tokens} "
                                                      f"rows and a cache of {self.kv_heads} heads of {self.head_dim}, on one device")
         hq = hkv
         if q is not None:
             hq = q.shape[1]
-            if q.shape != (n, hq, d) or q.dtype != k.dtype:
-                raise FusorHipError(_lib.FH_ERR_INVALID, f"q {q.shape} {q.dtype} does not match k {k.shape} {k.dtype}")
+            if q.shape != (n, hq, d) or q.dtype != k.dtype or q.device is not self.device:
+                raise FusorHipError(_lib.FH_ERR_INVALID, f"q {q.shape} {q.dtype} does not match k {k.shape} {k.dtype}, on one device")
             if out is None:
                 out = Tensor(self.device, q.shape, q.dtype)
-            elif out.shape != q.shape or out.dtype != q.dtype:
-                raise FusorHipError(_lib.FH_ERR_INVALID, f"out is {q.dtype} {q.shape}, not {out.dtype} {out.shape}")
+            elif out.shape != q.shape or out.dtype != q.dtype or out.device is not self.device:
+                raise FusorHipError(_lib.FH_ERR_INVALID, f"out is {q.dtype} {q.shape} of the rows' device, not {out.dtype} {out.shape}")
         cos, sin, rows, pairs, axes, sec = None, None, 0, 0, 1, None
         if rope is not None:
+            if rope.cos.device is not self.device or rope.sin.device is not self.device:
+                raise FusorHipError(_lib.FH_ERR_INVALID, "the rotation's tables are on another device than the pages")
             cos, sin, (rows, pairs) = rope.cos.ptr, rope.sin.ptr, rope.cos.shape
             if sections is not None:
                 axes, sec = len(sections), (C.c_int32 * len(sections))(*sections)
-            if positions is not None and (positions.dtype != "i32" or positions.shape != (axes, n)):
-                raise FusorHipError(_lib.FH_ERR_INVALID, f"positions are i32 {(axes, n)}, not {positions.dtype} {positions.shape}")
+            if positions is not None and (positions.dtype != "i32" or positions.shape != (axes, n) or positions.device is not self.device):
+                raise FusorHipError(_lib.FH_ERR_INVALID, f"positions are i32 {(axes, n)} of the rows' device, not {positions.dtype} {positions.shape}")
         st, sh = strides or (0, d)
         L = self.device._lib
         status = L.fh_paged_rope_append(self.device._h, _ELEMENTS[k.dtype], self.code, None if q is None else q.ptr, st or hq * d, sh,

@@ -1,0 +1,80 @@
+"""What the paged operators of the Python surface refuse before they call the library: on devices that are none, with made-up pointers."""
+import pytest
+
+from kalosm_amd.fusor import FusorHipError, PagedBatch, PagedKvCache, RopeCache, Tensor
+
+
+class Nowhere:
+    """A device whose calls end the test: nothing here gets that far."""
+    _h = None
+
+    def alloc(self, size):
+        return 4096
+
+    def free(self, ptr):
+        pass
+
+    class _lib:
+        def __getattr__(self, name):
+            raise AssertionError(f"{name} was called")
+
+    _lib = _lib()
+
+
+HERE, THERE = Nowhere(), Nowhere()
+
+
+def t(*shape, dtype="f16", device=HERE):
+    return Tensor(device, shape, dtype, ptr=4096)
+
+
+def i32(*shape, device=HERE):
+    return t(*shape, dtype="i32", device=device)
+
+
+def given(**other):
+    """The arguments of a call that is right, on HERE but for those named."""
+    at = {name: other.get(name, HERE) for name in ("q", "k", "v", "out", "cache", "batch", "positions", "cos", "sin")}
+    d = {name: t(3, 8, 64, device=at[name]) for name in ("q", "out")}
+    d.update({name: t(3, 2, 64, device=at[name]) for name in "kv"})
+    d["cache"] = PagedKvCache.over(t(9, 2, 16, 64, device=at["cache"]), t(9, 2, 16, 64, device=at["cache"]))
+    d["batch"] = PagedBatch(i32(3, device=at["batch"]), i32(3, 4, device=at["batch"]))
+    d["positions"] = i32(1, 3, device=at["positions"])
+    d["rope"] = RopeCache.__new__(RopeCache)
+    d["rope"].device, d["rope"].cos, d["rope"].sin = at["cos"], t(32, 32, dtype="f32", device=at["cos"]), t(32, 32, dtype="f32", device=at["sin"])
+    return d
+
+
+def attention(d):
+    d["q"].paged_attention(d["cache"], d["batch"], 0.1, out=d["out"])
+
+
+def append(d):
+    d["cache"].append(d["k"], d["v"], d["batch"])
+
+
+def turned(d):
+    d["rope"].forward_paged(d["q"], d["k"], d["v"], d["cache"], d["batch"], d["positions"], out=d["out"])
+
+
+@pytest.mark.parametrize("call", [attention, append, turned])
+def test_what_is_right_reaches_the_library(call):
+    with pytest.raises(AssertionError, match="was called"):
+        call(given())
+
+
+@pytest.mark.parametrize("call,names", [(attention, ("q", "out", "cache", "batch")), (append, ("k", "v", "cache", "batch")),
+                                        (turned, ("q", "k", "v", "out", "cache", "batch", "positions", "cos", "sin"))])
+def test_tensors_of_another_device(call, names):
+    """Another handle is another stream, and may be another GPU: no order between its work and the call's."""
+    for name in names:
+        with pytest.raises(FusorHipError, match="device"):
+            call(given(**{name: THERE}))
+
+
+def test_a_batch_and_a_cache_are_of_one_device():
+    for lens, table, starts in ((THERE, HERE, HERE), (HERE, THERE, HERE), (HERE, HERE, THERE)):
+        with pytest.raises(FusorHipError, match="device"):
+            PagedBatch(i32(3, device=lens), i32(3, 4, device=table), i32(4, device=starts), tokens=5)
+    with pytest.raises(FusorHipError, match="device"):
+        PagedKvCache.over(t(9, 2, 16, 64), t(9, 2, 16, 64, device=THERE))
