@@ -522,6 +522,8 @@ class RopeCache:
 
     def __init__(self, device: Device, cos: Tensor, sin: Tensor):
         self.device, self.cos, self.sin = device, cos, sin
+        if cos.dtype != "f32" or sin.dtype != "f32" or sin.nbytes < cos.nbytes:  # (both are read as f32 of the cosines' shape)
+            raise FusorHipError(_lib.FH_ERR_INVALID, f"a rotation's tables are f32, both alike, not {cos.dtype} {cos.shape} and {sin.dtype} {sin.shape}")
 
     @staticmethod
     def new(head_dim: int, context_length: int, rope_theta: float, device: Device) -> "RopeCache":
@@ -694,9 +696,12 @@ class PagedKvCache:
                 raise FusorHipError(_lib.FH_ERR_INVALID, f"out is {q.dtype} {q.shape} of the rows' device, not {out.dtype} {out.shape}")
         cos, sin, rows, pairs, axes, sec = None, None, 0, 0, 1, None
         if rope is not None:
-            if rope.cos.device is not self.device or rope.sin.device is not self.device:
+            cos, sin = rope.cos, rope.sin
+            if cos.device is not self.device or sin.device is not self.device:
                 raise FusorHipError(_lib.FH_ERR_INVALID, "the rotation's tables are on another device than the pages")
-            cos, sin, (rows, pairs) = rope.cos.ptr, rope.sin.ptr, rope.cos.shape
+            if len(cos.shape) != 2 or sin.shape != cos.shape or cos.dtype != "f32" or sin.dtype != "f32":
+                raise FusorHipError(_lib.FH_ERR_INVALID, f"a rotation's tables are f32 [positions, pairs], both alike, not {cos.dtype} {cos.shape} and {sin.dtype} {sin.shape}")
+            cos, sin, (rows, pairs) = cos.ptr, sin.ptr, cos.shape
             if sections is not None:
                 axes, sec = len(sections), (C.c_int32 * len(sections))(*sections)
             if positions is not None and (positions.dtype != "i32" or positions.shape != (axes, n) or positions.device is not self.device):

@@ -78,3 +78,15 @@ def test_a_batch_and_a_cache_are_of_one_device():
             PagedBatch(i32(3, device=lens), i32(3, 4, device=table), i32(4, device=starts), tokens=5)
     with pytest.raises(FusorHipError, match="device"):
         PagedKvCache.over(t(9, 2, 16, 64), t(9, 2, 16, 64, device=THERE))
+
+
+@pytest.mark.parametrize("cos,sin", [(t(32, 32), t(32, 32)), (t(32, 32, dtype="f32"), t(32, 32)), (t(32, 32, dtype="f32"), t(31, 32, dtype="f32")),
+                                     (t(32, 32, dtype="f32"), t(32, 16, dtype="f32")), (t(1024, dtype="f32"), t(1024, dtype="f32"))])
+def test_tables_that_are_not_read_past_their_end(cos, sin):
+    d = given()
+    d["rope"].cos, d["rope"].sin = cos, sin  # (put there afterwards)
+    with pytest.raises(FusorHipError, match="tables are f32"):
+        turned(d)
+    if sin.nbytes < cos.nbytes or "f16" in (cos.dtype, sin.dtype):
+        with pytest.raises(FusorHipError, match="tables are f32"):
+            RopeCache.from_parts(cos, sin)
