@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from operator import attrgetter
 from typing import Optional, Sequence
 
 import numpy as np
@@ -361,7 +362,7 @@ class Tensor:
         positions where that is not 0.  `strides` = (row, head) element strides of a view (of a fused projection's rows,
         say) whose logical shape is self.shape.  The keys and values of the rows themselves must have been appended."""
         tokens, hq, d = self.shape
-        if tokens != batch.tokens or d != cache.head_dim or self.dtype not in _ELEMENTS or self.device is not cache.device or batch.device is not cache.device:
+        if tokens != batch._tokens or d != cache._head_dim or self.dtype not in _ELEMENTS or self.device is not cache._device or batch._device is not cache._device:
             raise FusorHipError(_lib.FH_ERR_INVALID, f"rows of shape {self.shape} ({self.dtype}) do not match a batch of {batch.tokens} rows "
                                                      f"and a cache of head_dim {cache.head_dim}, on one device")
         if out is None:
@@ -370,8 +371,8 @@ class Tensor:
             raise FusorHipError(_lib.FH_ERR_INVALID, f"out is {self.dtype} {self.shape} of the rows' device, not {out.dtype} {out.shape}")
         st, sh = strides or (hq * d, d)
         L = self.device._lib
-        status = L.fh_paged_attention(self.device._h, _ELEMENTS[self.dtype], cache.code, self.ptr, st, sh, hq, cache.kv_heads, d,
-                                      scale, window, *cache.layer(layer), *batch.args, batch.max_new, batch.max_len, out.ptr)
+        status = L.fh_paged_attention(self.device._h, _ELEMENTS[self.dtype], cache._code, self.ptr, st, sh, hq, cache._kv_heads, d,
+                                      scale, window, *cache.layer(layer), *batch._args, batch.max_new, batch.max_len, out.ptr)
         if status:
             check(status)
         return out
@@ -618,13 +619,20 @@ class KvCache:
             pass
 
 
+def _fixed(name: str) -> property:
+    """An attribute that is given once: what the calls take was made from it."""
+    return property(attrgetter("_" + name))
+
+
 class PagedBatch:
     """Which rows of a call belong to which sequence, and the pages of every sequence: device tensors that the calls read
     when they run, so a program (or a captured graph) fills in new lengths and pages between them (other tensors are another batch).
 
     lens [n] i32: positions of every sequence, its new rows among them.  table [n, columns] i32: its pages.  starts [n + 1]
     i32: sequence i has the rows starts[i] .. starts[i + 1] - 1; None: one row each.  tokens: rows of the tensors.  max_new:
-    the most new rows of a sequence.  max_len: the longest of lens where the host knows it (0: no matter)."""
+    the most new rows of a sequence.  max_len: the longest of lens where the host knows it (0: no matter).  These two may be set anew."""
+
+    device, lens, table, starts, tokens, args = map(_fixed, ("device", "lens", "table", "starts", "tokens", "args"))
 
     def __init__(self, lens: Tensor, table: Tensor, starts: Optional[Tensor] = None, tokens: Optional[int] = None,
                  max_new: Optional[int] = None, max_len: int = 0):
@@ -634,18 +642,21 @@ class PagedBatch:
                 raise FusorHipError(_lib.FH_ERR_INVALID, f"{what} is i32 {shape} of the table's device, not {t.dtype} {t.shape}")
         if starts is not None and tokens is None:
             raise FusorHipError(_lib.FH_ERR_INVALID, "a batch with starts needs its number of rows")
-        self.device, self.lens, self.table, self.starts = table.device, lens, table, starts
-        self.tokens = n if tokens is None else int(tokens)
-        self.max_new = (1 if starts is None else self.tokens) if max_new is None else int(max_new)
+        self._device, self._lens, self._table, self._starts = table.device, lens, table, starts
+        self._tokens = n if tokens is None else int(tokens)
+        self.max_new = (1 if starts is None else self._tokens) if max_new is None else int(max_new)
         self.max_len = int(max_len)
         # (as the calls take them: made once, not converted again in each)
-        self.args = (C.c_void_p(None if starts is None else starts.ptr), C.c_void_p(lens.ptr), C.c_void_p(table.ptr), C.c_int32(cols), C.c_int32(n),
-                     C.c_int32(self.tokens))
+        self._args = (C.c_void_p(None if starts is None else starts.ptr), C.c_void_p(lens.ptr), C.c_void_p(table.ptr), C.c_int32(cols), C.c_int32(n),
+                      C.c_int32(self._tokens))
 
 
 class PagedKvCache:
     """Keys and values of many sequences in pages, `layers` layers at once: k and v [layers, pages, kv_heads, page_size,
     head_dim].  Which page holds what is the caller's: a PagedBatch names the pages of its sequences."""
+
+    device, k, v, dtype, code = map(_fixed, ("device", "k", "v", "dtype", "code"))
+    layers, pages, kv_heads, page_size, head_dim = map(_fixed, ("n_layers", "pages", "kv_heads", "page_size", "head_dim"))
 
     def __init__(self, device: Device, layers: int, kv_heads: int, head_dim: int, pages: int, page_size: int, dtype: str = "f16"):
         shape = (layers, pages, kv_heads, page_size, head_dim)
@@ -662,17 +673,16 @@ class PagedKvCache:
         shape = k.shape if len(k.shape) == 5 else (1, *k.shape)
         if len(shape) != 5 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _ELEMENTS or v.device is not k.device:
             raise FusorHipError(_lib.FH_ERR_INVALID, f"pages of shapes {k.shape}, {v.shape} and types {k.dtype}, {v.dtype}, on one device")
-        self.device, self.k, self.v, self.dtype, self.code = k.device, k, v, k.dtype, _ELEMENTS[k.dtype]
-        self.layers, self.pages, self.kv_heads, self.page_size, self.head_dim = shape
-        row = self.page_size * self.head_dim
-        step = k.nbytes // self.layers
-        sizes = (C.c_int64(self.kv_heads * row), C.c_int64(row), C.c_int64(self.head_dim), C.c_int32(self.pages), C.c_int32(self.page_size))
-        self._layers = [(C.c_void_p(k.ptr + i * step), C.c_void_p(v.ptr + i * step), *sizes) for i in range(self.layers)]
+        self._device, self._k, self._v, self._dtype, self._code = k.device, k, v, k.dtype, _ELEMENTS[k.dtype]
+        self._n_layers, self._pages, self._kv_heads, self._page_size, self._head_dim = n, pages, heads, size, d = shape
+        step = k.nbytes // n
+        sizes = (C.c_int64(heads * size * d), C.c_int64(size * d), C.c_int64(d), C.c_int32(pages), C.c_int32(size))
+        self._layers = [(C.c_void_p(k.ptr + i * step), C.c_void_p(v.ptr + i * step), *sizes) for i in range(n)]
 
     def layer(self, layer: int):
         """A layer's pointers, strides and sizes as the library takes them."""
-        if not 0 <= layer < self.layers:
-            raise FusorHipError(_lib.FH_ERR_INVALID, f"layer {layer} of {self.layers}")
+        if not 0 <= layer < len(self._layers):
+            raise FusorHipError(_lib.FH_ERR_INVALID, f"layer {layer} of {len(self._layers)}")
         return self._layers[layer]
 
     def append(self, k: Tensor, v: Tensor, batch: PagedBatch, layer: int = 0, strides: Optional[Sequence[int]] = None) -> None:
@@ -681,37 +691,37 @@ class PagedKvCache:
 
     def _append(self, rope, q, k, v, batch, positions, sections, interleaved, layer, strides, out):
         n, hkv, d = k.shape
-        if k.shape != v.shape or k.dtype != v.dtype or n != batch.tokens or hkv != self.kv_heads or d != self.head_dim \
-                or k.dtype not in _ELEMENTS or k.device is not self.device or v.device is not self.device or batch.device is not self.device:
+        if k.shape != v.shape or k.dtype != v.dtype or n != batch._tokens or hkv != self._kv_heads or d != self._head_dim \
+                or k.dtype not in _ELEMENTS or k.device is not self._device or v.device is not self._device or batch._device is not self._device:
             raise FusorHipError(_lib.FH_ERR_INVALID, f"k {k.shape} ({k.dtype}) and v {v.shape} ({v.dtype}) do not match a batch of {batch.tokens} "
                                                      f"rows and a cache of {self.kv_heads} heads of {self.head_dim}, on one device")
         hq = hkv
         if q is not None:
             hq = q.shape[1]
-            if q.shape != (n, hq, d) or q.dtype != k.dtype or q.device is not self.device:
+            if q.shape != (n, hq, d) or q.dtype != k.dtype or q.device is not self._device:
                 raise FusorHipError(_lib.FH_ERR_INVALID, f"q {q.shape} {q.dtype} does not match k {k.shape} {k.dtype}, on one device")
             if out is None:
-                out = Tensor(self.device, q.shape, q.dtype)
-            elif out.shape != q.shape or out.dtype != q.dtype or out.device is not self.device:
+                out = Tensor(self._device, q.shape, q.dtype)
+            elif out.shape != q.shape or out.dtype != q.dtype or out.device is not self._device:
                 raise FusorHipError(_lib.FH_ERR_INVALID, f"out is {q.dtype} {q.shape} of the rows' device, not {out.dtype} {out.shape}")
         cos, sin, rows, pairs, axes, sec = None, None, 0, 0, 1, None
         if rope is not None:
             cos, sin = rope.cos, rope.sin
-            if cos.device is not self.device or sin.device is not self.device:
+            if cos.device is not self._device or sin.device is not self._device:
                 raise FusorHipError(_lib.FH_ERR_INVALID, "the rotation's tables are on another device than the pages")
             if len(cos.shape) != 2 or sin.shape != cos.shape or cos.dtype != "f32" or sin.dtype != "f32":
                 raise FusorHipError(_lib.FH_ERR_INVALID, f"a rotation's tables are f32 [positions, pairs], both alike, not {cos.dtype} {cos.shape} and {sin.dtype} {sin.shape}")
             cos, sin, (rows, pairs) = cos.ptr, sin.ptr, cos.shape
             if sections is not None:
                 axes, sec = len(sections), (C.c_int32 * len(sections))(*sections)
-            if positions is not None and (positions.dtype != "i32" or positions.shape != (axes, n) or positions.device is not self.device):
+            if positions is not None and (positions.dtype != "i32" or positions.shape != (axes, n) or positions.device is not self._device):
                 raise FusorHipError(_lib.FH_ERR_INVALID, f"positions are i32 {(axes, n)} of the rows' device, not {positions.dtype} {positions.shape}")
         st, sh = strides or (0, d)
-        L = self.device._lib
-        status = L.fh_paged_rope_append(self.device._h, _ELEMENTS[k.dtype], self.code, None if q is None else q.ptr, st or hq * d, sh,
+        L = self._device._lib
+        status = L.fh_paged_rope_append(self._device._h, _ELEMENTS[k.dtype], self._code, None if q is None else q.ptr, st or hq * d, sh,
                                         k.ptr, v.ptr, st or hkv * d, sh, hq, hkv, d, cos, sin, rows, pairs,
                                         None if positions is None else positions.ptr, sec, axes, int(interleaved), *self.layer(layer),
-                                        *batch.args, None if q is None else out.ptr)
+                                        *batch._args, None if q is None else out.ptr)
         if status:
             check(status)
         return out if q is not None else None

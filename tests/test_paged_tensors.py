@@ -90,3 +90,19 @@ def test_tables_that_are_not_read_past_their_end(cos, sin):
     if sin.nbytes < cos.nbytes or "f16" in (cos.dtype, sin.dtype):
         with pytest.raises(FusorHipError, match="tables are f32"):
             RopeCache.from_parts(cos, sin)
+
+
+def test_what_the_calls_were_made_from_stays():
+    """A batch and a cache hold pointers and sizes made from their tensors: other tensors or sizes are another batch or cache."""
+    d = given()
+    for whose, names in (("batch", ("device", "lens", "table", "starts", "tokens", "args")), ("cache", ("device", "k", "v", "dtype", "code", "layers", "pages", "kv_heads", "page_size", "head_dim"))):
+        for name in names:
+            before = getattr(d[whose], name)
+            with pytest.raises(AttributeError):
+                setattr(d[whose], name, i32(3))
+            assert getattr(d[whose], name) is before
+    batch, cache = d["batch"], d["cache"]
+    assert (batch.tokens, batch.lens.shape, batch.table.shape, batch.starts) == (3, (3,), (3, 4), None)
+    assert (cache.layers, cache.pages, cache.kv_heads, cache.page_size, cache.head_dim, cache.dtype, cache.k.shape) == (1, 9, 2, 16, 64, "f16", (9, 2, 16, 64))
+    batch.max_new, batch.max_len = 2, 40  # (these are looked at in every call)
+    assert (batch.max_new, batch.max_len) == (2, 40)
