@@ -63,6 +63,7 @@ __device__ __forceinline__ float paged_brought(float scale, int &ex) {
 template <typename TX, typename TP>
 __device__ __forceinline__ void paged_again(const TX *q, int d, float sc2, float shift, const PagedKv &kv, const int *table, int kh, int from, int to, float &m, float &l,
                                             float (&o)[4]) {
+    constexpr float SMALLER = __is_same(TP, fh_half) ? 0x1p-24f : 1.f; // (f32 rows times f16 keys: 2^127 * 2^16 * 256; keys of the other types can be as large as rows are small)
     const int lane = threadIdx.x & 63;
     m = -INFINITY, l = 0.f;
     for (int e = 0; e < 4; e++) o[e] = 0.f;
@@ -81,9 +82,9 @@ __device__ __forceinline__ void paged_again(const TX *q, int d, float sc2, float
                     uint4 w[sizeof(TP) / 2];
                     for (int i = 0; i < (int)sizeof(TP) / 2; i++) w[i] = ((const uint4 *)(kv.k + at + e * (int)sizeof(TP)))[i];
                     __builtin_memcpy(x, w, sizeof(x));
-                    for (int i = 0; i < 8; i++) y = fmaf((float)q[e + i] * 0x1p-24f, (float)x[i], y); // (f16 keys next to f32 rows: 2^127 * 2^16 * 256)
+                    for (int i = 0; i < 8; i++) y = fmaf((float)q[e + i] * SMALLER, (float)x[i], y);
                 }
-                y *= sc2 * 0x1p24f;
+                y *= sc2 / SMALLER;
             }
         }
         float mx = y;

@@ -1,4 +1,5 @@
-"""f32 rows over f16 pages, which go to the matrix cores brought to 2^14 by a power of two that the scale takes back: rows and scales of any size."""
+"""Rows and scales of any size: f32 rows over f16 pages, which go to the matrix cores brought to 2^14 by a power of two that the scale takes back, and rows as small as
+keys are large."""
 import numpy as np
 import pytest
 
@@ -79,3 +80,23 @@ def test_large_rows_in_front_of_what_they_do_not_see(dev, d, new, lens):
         top = int(np.argmax(k[p.table[i, j // 16], 0, j % 16, 5]))
         o = np.repeat(v[p.table[i, top // 16], :, top % 16], 2, 0)
         near(got[row], o, attention_bound(o, np.abs(o), 0 * o, 0.0, last + 1, d, "f32", "f16"), f"row {row}")
+
+
+@pytest.mark.parametrize("act,kept", [("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("d", [64, 128, 200])
+@pytest.mark.parametrize("new,lens", [([4] * 9, [60] * 9), ([70, 20], [300, 90]), ([20], [3000])])
+def test_small_rows_in_front_of_what_they_do_not_see(dev, act, kept, d, new, lens):
+    """q of 2^-124 and keys of 2^124, both of 8 bits: scores of some units, worked out again where only the last row looks at infinities."""
+    p = Pages(11, new, lens, 4, 2, d, 16, act, kept)
+    rng = np.random.default_rng(12)
+    some = [rng.choice([-1, 1], s) * rng.integers(128, 256, s) / 128 for s in (p.q.shape, p.k.shape)]
+    k, v = 2.0 ** 124 * some[1], unpack(p.v, kept)
+    for i, n in enumerate(lens):
+        v[p.table[i, (n - 1) // 16], :, (n - 1) % 16, 1] = np.inf
+    p.q, p.k, p.v = pack(2.0 ** -124 * some[0], act), pack(k, kept), pack(v, kept)
+    got = run(dev, p, 0.125)
+    with np.errstate(invalid="ignore"):
+        want, bound = p.attention(0.125)
+    fine = np.isfinite(want)
+    assert (~fine).sum() == 4 * len(lens) and (np.isfinite(got) == fine).all()
+    near(got[fine], want[fine], bound[fine], f"{act}/{kept} {new[:2]}")
