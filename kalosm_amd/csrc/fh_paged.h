@@ -49,6 +49,13 @@ __device__ __forceinline__ PagedSeq paged_seq_scalar(const PagedRows &r, int shi
     return r.starts ? paged_seq(r, shift, len, paged_scalar(r.starts, i), paged_scalar(r.starts, i + 1)) : paged_seq(r, shift, len, i, i + 1);
 }
 
+// The first of an f32 value's terms, what is left is the next ones': rounded, but to bf16's largest value what would be rounded to infinity (infinities and NaN stay in
+// what is left).
+template <typename T> __device__ __forceinline__ T paged_first(float x) {
+    if constexpr (__is_same(T, fh_bf)) x = fminf(fmaxf(x, -0x1.fep127f), 0x1.fep127f);
+    return (T)x;
+}
+
 // The scale of scores whose row is taken 2^ex times as large.  It stays a normal number - ex is no larger than that allows, and scores of smaller rows do not tell
 // positions apart: they are below 2^(15 + 16 + 8 - 126) - and finite: where it would not be, scores are 0 or, of the smallest key, 2^(14 - 24 + 128) apart.
 __device__ __forceinline__ float paged_brought(float scale, int &ex) {

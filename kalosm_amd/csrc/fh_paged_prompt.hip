@@ -482,7 +482,7 @@ __global__ __launch_bounds__(256) void k_paged_planes(PpArgs a) {
             for (int u = 0; u < QT; u++)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const T y = (T)v[e];
+                    const T y = u == 0 && QT > 1 ? paged_first<T>(v[e]) : (T)v[e];
                     qf[u][ks][e] = y;
                     v[e] -= (float)y;
                 }

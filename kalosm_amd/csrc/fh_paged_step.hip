@@ -315,7 +315,7 @@ __global__ __launch_bounds__(64 * NWV) void k_paged_step(const int *__restrict__
                     for (int u = 0; u < QT; u++)
 #pragma unroll
                         for (int e = 0; e < E; e++) {
-                            const TP v = (TP)x[s][e];
+                            const TP v = u == 0 && QT > 1 ? paged_first<TP>(x[s][e]) : (TP)x[s][e];
                             qf[u][s][e] = v;
                             x[s][e] -= (float)v;
                         }

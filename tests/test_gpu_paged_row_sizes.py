@@ -100,3 +100,25 @@ def test_small_rows_in_front_of_what_they_do_not_see(dev, act, kept, d, new, len
     fine = np.isfinite(want)
     assert (~fine).sum() == 4 * len(lens) and (np.isfinite(got) == fine).all()
     near(got[fine], want[fine], bound[fine], f"{act}/{kept} {new[:2]}")
+
+
+@pytest.mark.parametrize("kept", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 200])
+@pytest.mark.parametrize("new,lens", BATCHES)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_rows_of_the_largest_floats(dev, kept, d, new, lens, sign):
+    """Rows of f32's largest value, which bf16 would round to infinity: keys of 0 have scores of 0, and one of 2^-100 has 2^28 or -2^28, without end apart from them."""
+    p = Pages(13, new, lens, 4, 2, d, 16, "f32", kept)
+    v, k = unpack(p.v, kept), np.zeros(p.k.shape)
+    first = [(n - m) // 2 for m, n in zip(new, lens)]
+    for i, at in enumerate(first):
+        k[p.table[i, at // 16], :, at % 16, 3] = sign * 2.0 ** -100
+    p.k, p.q = pack(k, kept), np.full(p.q.shape, np.finfo(np.float32).max, np.float32)
+    got = run(dev, p, 1.0)
+    for row, i, last in p.rows():
+        j = np.arange(last + 1)
+        if last >= first[i]:
+            j = np.array([first[i]]) if sign > 0 else np.delete(j, first[i]) if last else j
+        x = v[p.table[i, j // 16], :, j % 16]
+        o, mass, whole = (np.repeat(y, 2, 0) for y in (x.mean(0), np.abs(x).mean(0), np.abs(x).sum(0)))
+        near(got[row], o, attention_bound(o, mass, whole, 0.0, last + 1, d, "f32", kept), f"row {row}")
