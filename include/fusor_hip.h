@@ -312,8 +312,9 @@ fh_status fh_flash_attention_decode_static(fh_device *dev, int32_t q_dtype, int3
  * [page][slot][head]).  The pages are the caller's memory: nothing is allocated or kept here.  No counterpart in the
  * reference, whose cache is one dense sequence (fusor-ml/fusor/src/cache/kv_cache.rs:24-63).
  *   rows     tokens of all sequences one after the other: starts_dev[i] .. starts_dev[i + 1] - 1 are the new ones of
- *            sequence i (i32, seqs + 1 of them, not decreasing; NULL: one row each).  Rows before the first and behind the
- *            last sequence are left as they were, in the pages and in the outputs.
+ *            sequence i (i32, seqs + 1 of them from 0 to `tokens`, not decreasing; NULL: one row each).  Rows before the
+ *            first and behind the last sequence are left as they were, in the pages and in the outputs.  Starts that are
+ *            not like that read and write nothing out of bounds; which positions their rows have is not said.
  *   lens_dev positions of every sequence, its new rows among them (i32): row r has position
  *            lens[i] - (starts[i + 1] - r).
  *   table_dev [seqs, table_cols] i32: the page of positions n * page_size .. is table[i][n].  An entry that is no page
@@ -325,7 +326,9 @@ fh_status fh_flash_attention_decode_static(fh_device *dev, int32_t q_dtype, int3
  * Infinities and NaN among the keys and values that a row sees may make its results infinities or NaN; what it does not
  * see (later rows, positions before its window, slots that no position has reached) makes no difference, whatever it is.
  * Results are f32 sums of the values, each times a weight of up to 2^8 (next to f16: 2^16), over the sum of the weights:
- * where f32 or bf16 values are so large that these sums pass 2^128, the results are infinities.
+ * where f32 or bf16 values are so large that these sums pass 2^128, the results are infinities or NaN; and so where
+ * scores do, or next to bf16 and f32 pages the sums q . k before their scale.  f32 values below 2^-100 may lose bits next
+ * to bf16 pages and in prompts over f32 pages, where they are sums of bf16 terms.
  * Sequences may share pages: what one appends the others see, and a slot that two rows of one call are appended to holds
  * pieces of either.
  * At most 65535 heads and sequences, and 2^29 positions of a sequence, rows and pages. */
@@ -333,7 +336,8 @@ fh_status fh_flash_attention_decode_static(fh_device *dev, int32_t q_dtype, int3
 /* q and k turned by their positions (RopeCache::forward{,_interleaved}, fusor-ml/fusor/src/composite/rope.rs:284-329; with
  * several axes as models/kalosm-llama/src/raw/rope.rs does for pictures), k and v written to their pages.  q is
  * [tokens, hq, d] with strides q_st (row) and q_sh (head) in elements, k and v are [tokens, hkv, d] with kv_st and kv_sh;
- * q_out is contiguous [tokens, hq, d].  q and q_out may be NULL (append only), and cos and sin (nothing turns).
+ * q_out is contiguous [tokens, hq, d].  q and q_out may be NULL (append only; hq is a multiple of hkv all the same), and cos
+ * and sin (nothing turns).
  * cos / sin: [table_rows, table_pairs] f32.  Pair j of a head takes column j of the row that its axis' position names:
  * sections_host[axes] (1 .. 4 axes) says how many pairs follow each axis, the first ones axis 0; NULL with one axis: all
  * table_pairs.  What the sections leave of a head is not turned.  positions_dev: [axes, tokens] i32, NULL with one axis: the

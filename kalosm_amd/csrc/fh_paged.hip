@@ -124,7 +124,7 @@ template <typename T> __device__ __forceinline__ void paged_store8(T *p, const f
 
 // A thread takes eight pairs of a head, or eight values that are copied (V, what the sections leave): moves 4 to 6 bytes an operation, so it is bound by the
 // memory for many rows, and by the chain of requests for few: the values are asked for before the row's place is looked up.
-// (32 / 8 heads of 128: 1 row of f32 2.8 us, 64 of bf16 3.7, 22 thousand of f16 by three axes 106, 5.2 TB/s.)
+// (32 / 8 heads of 128: 1 row of f32 2.8 us, 64 of bf16 3.7, 22 thousand of f16 by three axes 97 to 106, 5.2 to 5.7 TB/s.)
 // grid (rows, units of a row / 256)
 template <typename TX, typename TP, bool TANGLED>
 __global__ __launch_bounds__(256) void k_paged_append8(const TX *q, const TX *__restrict__ k, const TX *__restrict__ v, int hq, int hkv, int d, int n,

@@ -8,8 +8,8 @@
 // A page's 16 positions are one scalar address: requests add a lane's constant offset.
 // grid (KV heads, blocks of rows - the last, longest ones first -, sequences x parts).  With fewer workgroups than compute units the
 // positions are split over `parts` workgroups, whose sums go to scratch memory in f32 and are added up by a second launch.
-// Measured (32 / 8 heads of 128): 8192 tokens of f16 605 to 645 us by the card, 855 to 910 TFLOP/s, the matrix cores busy 44 % of the cycles; 8 sequences of
-// 184 to 512 behind up to 4001, bf16, 179 us, 740; 33 behind 65536, f16, 90 us, 3.0 TB/s (a workgroup has one step of 64 KB on its way, which takes 2.3 us
+// Measured (32 / 8 heads of 128): 8192 tokens of f16 605 to 651 us by the card, 845 to 910 TFLOP/s, the matrix cores busy 45 % of the cycles; 8 sequences of
+// 184 to 512 behind up to 4001, bf16, 174 to 185 us, 715 to 760; 33 behind 65536, f16, 90 us, 3.0 TB/s (a workgroup has one step of 64 KB on its way, which takes 2.3 us
 // whatever the number of rows).  2 x 2049, window 1024, 16 / 4 heads of 64, f32: 104 us, 110 TFLOP/s.
 //
 // Positions that a row does not see have weight 0, whatever lies there: scores are replaced, and where a row's sums end up infinite or NaN and a position in its
@@ -432,6 +432,8 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(2, 2))
 // Tiles of 32 positions through registers into LDS, f32 pages as three bf16 planes that add up to their values (24 bits, the whole range); f32 rows
 // as three terms of bf16, or two of f16 brought to 2^14 first (22 bits).  Products of terms beyond the third order are below 2^-24 and left out:
 // six where both operands have three, three or two where pages are of 16 bits.  Weights have as many terms as Q.
+// One buffer, two barriers a tile: products, softmax and splitting follow each other (2048 rows, us, 32 / 8 heads of 128: f32 231, f32 over f16 130, over bf16 133; 16 / 4 heads
+// of 256: f16 147, bf16 129, f32 523, over f16 185, over bf16 297).
 template <typename TX, typename TP, int DP>
 __global__ __launch_bounds__(256) void k_paged_planes(PpArgs a) {
     constexpr bool F32 = sizeof(TP) == 4, F16 = __is_same(TP, fh_half), MIXED = sizeof(TX) != sizeof(TP);

@@ -20,8 +20,9 @@
 // each with its own running maximum and sum, and are joined through LDS where the pair (or the stretch) ends.  What is not a
 // whole pair goes to scratch memory, two places a workgroup, and whoever of the pair's workgroups counts itself in last adds
 // them up, in their order: the same bits in every run.  Pairs of few tiles are a workgroup each, and nothing is joined.
-// Measured (32 / 8 heads of 128; a copy: 4.6 TB/s): 1 sequence of 131072, bf16, 101 us, 5.3 TB/s; 64 of 8192, f32 rows over f16, 64 / 8 heads, 243 us, 5.5;
-// 32 of 2048, f16, a pair a workgroup, 38 us, 4.5.  1 of 300, f32: 12 us, bound by the f32 products of eight compute units and their requests.
+// Measured (32 / 8 heads of 128; a copy: 4.6 TB/s): 1 sequence of 131072, bf16, 98 to 101 us, 5.3 to 5.5 TB/s; 64 of 8192, f32 rows over f16, 64 / 8 heads, 235 to 245 us, 5.5 to 5.7;
+// 32 of 2048, f16, a pair a workgroup, 38 us, 4.5.  1 of 300, f32: 12 us, by eight workgroups, each through its
+// products and requests one behind the other; the dense cache's kernel, over more compute units and with a second launch, takes 6.8.
 #include "fh_paged.h"
 #include <type_traits>
 
